@@ -87,6 +87,24 @@ typedef struct w4b_kv_f8 {
   const uint16_t* s_v;
 } w4b_kv_f8;
 
+/* Value types of activations where an entry takes more than FP16. */
+#define W4B_DTYPE_F16 0
+#define W4B_DTYPE_BF16 1
+
+/* Paged 8-bit KV cache (no counterpart in the reference, whose FP8 cache is contiguous with a
+ * scale per position and group, include/w4/kvflash.cuh:390-396): H head slabs of npages * page
+ * rows of D E4M3 codes, and one FP32 scale per (head, page) for K and for V. Logical position t
+ * of a sequence is row bt[t/page]*page + t%page of every slab, its value code * scale[page].
+ * D 64 or 128; page a multiple of 16 up to 4096; scales positive, within 2^-60 .. 2^60. */
+typedef struct w4b_kv_b8 {
+  int H, D;
+  int page, npages;
+  uint8_t* q_k; /* [H][npages*page][D] */
+  float* s_k;   /* [H][npages] */
+  uint8_t* q_v;
+  float* s_v;
+} w4b_kv_b8;
+
 /* ---- library state ---------------------------------------------------- */
 
 const char* w4b_last_error(void);
@@ -272,6 +290,65 @@ int w4b_attn_single_fp16(const void* q, const void* k16, const void* v16, void* 
                          int D, void* stream);
 int w4b_attn_single_w4(const w4b_kv_w4* p, const void* q, void* out, void* stream, void* k_out,
                        void* v_out);
+
+/* ---- paged 8-bit cache: block tables, write, attention ------------------- */
+
+/* No counterpart in the reference. The three calls of a serving step over a paged cache whose
+ * lengths live on the device: the tables of the step, the write of the new tokens, attention.
+ * All three only launch on `stream` and may be captured into a graph.
+ *
+ * w4b_page_tables: block tables and slot maps from request lengths. Request i (of nseq <= 16384)
+ *   holds cached[i] positions and brings fresh[i] new tokens. Its new pages are taken from
+ *   free_pages[*taken_in ..] in request order and entered into its row of bt
+ *   (bt_stride ints per row; entries of pages it already holds are only read, entries behind its
+ *   last page are left as they are). Written: seq_lens[i] = cached[i] + fresh[i];
+ *   q_offsets[0..nseq], the exclusive sums of fresh; *taken_out = *taken_in + the new pages; and
+ *   for token t of the step (requests in order) positions[t] and
+ *   slots[t] = bt[position/page]*page + position%page, the row of every head slab; tokens behind
+ *   the last one, up to max_tokens, get slot -1 and position 0. seq_lens may be the array cached
+ *   and taken_out the word taken_in (a loop that advances in place). page is any size >= 1; the
+ *   tables serve every paged entry of this library. Faults of the values go to the device status
+ *   word: 601 when the free list ends early (the missing entries and their tokens' slots are -1,
+ *   *taken_out = nfree); 602 for a negative count, for a request longer than its table row or the
+ *   pool (it gets no pages, its tokens slot -1, its seq_lens 0), or when the tokens exceed
+ *   max_tokens (the first max_tokens are mapped).
+ * w4b_kv_write_b8: rows of T new tokens into the cache. k_new / v_new: FP16 or BF16 (dtype), token
+ *   t's H*D values at t * k_stride / t * v_stride values (multiples of 8, so a fused projection can
+ *   be passed as it is; bases 16-byte aligned). slots[t] is the token's row, -1 skips it. The tokens
+ *   that go to one page stand next to each other, in ascending slots without gaps, as
+ *   w4b_page_tables lays them out; no two requests write into the same page in one call. A run that
+ *   starts at row 0 of a page gives the page a new scale, the smallest power of two with
+ *   max|x| <= 448 * scale (2^-60 .. 2^60; larger values saturate); a run that continues a page keeps
+ *   the scale when its values fit and else raises it the same way and rounds the page's earlier
+ *   codes again. Rows behind the run keep their bytes. Status 501: a value that is not finite (that
+ *   token's row of that head is written as zeros) or too large; 603: a slot outside the pool, or a
+ *   page's tokens out of order (they are not written).
+ * w4b_attn_b8_paged: softmax(scale * q k^T) v over the cache for the new tokens of nseq sequences.
+ *   Hq query heads share the H cache heads in groups of Hq / H. Sequence i has seq_lens[i] <=
+ *   max_seq_len positions (its new tokens included) and query tokens q_offsets[i] ..
+ *   q_offsets[i+1] - 1, at most max_q of them (q_offsets NULL: one token each, max_q 1); with
+ *   causal != 0 its n tokens are its last n positions and see what is not behind them, without it
+ *   every token sees all positions (cross attention over an encoder's states: lengths of their
+ *   own). q / out: Hq*D values per token (dtype), a token every q_stride / out_stride values;
+ *   lse (optional) [token][Hq] FP32, the natural log of the sum of exponentials. A token that sees
+ *   nothing gets zeros and -inf. Rows of out outside the sequences' tokens are left as they are.
+ *   A block-table entry outside 0..npages-1 is read as a page without positions (status 604).
+ *   Lengths above max_seq_len and tokens above max_q are cut off there.
+ *   ws: w4b_attn_b8_workspace() bytes of device memory for this call (256-byte aligned, zero-filled
+ *   once by the caller; every call leaves the zeros it needs). Calls that may overlap - on two
+ *   streams, or two captured graphs - take different ones. NULL: library scratch, which is
+ *   allocated by the first such call (before any capture), never replaced, and shared by all of
+ *   them. Results do not depend on the other sequences' values; they are the same from run to run. */
+int w4b_page_tables(const int* cached, const int* fresh, int nseq, int page, int npages, const int* free_pages,
+                    int nfree, const int* taken_in, int* taken_out, int* bt, int bt_stride, int* seq_lens,
+                    int* q_offsets, int* slots, int* positions, int max_tokens, void* stream);
+int w4b_kv_write_b8(const w4b_kv_b8* p, const int* slots, int T, const void* k_new, const void* v_new,
+                    long long k_stride, long long v_stride, int dtype, void* stream);
+long long w4b_attn_b8_workspace(void);
+int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const int* seq_lens, const int* q_offsets,
+                      int nseq, int max_q, int max_seq_len, const void* q, long long q_stride, int Hq, int dtype,
+                      float scale, int causal, void* out, long long out_stride, float* lse, void* ws,
+                      long long ws_bytes, void* stream);
 
 /* ---- all-gather of the sharded GEMM's output over NVLink peer memory ----- */
 

@@ -18,6 +18,7 @@ from typing import Optional
 from . import build as _build
 
 PATH_AUTO, PATH_STREAM, PATH_TENSOR, PATH_GENERIC = 0, 1, 2, 3
+DTYPE_F16, DTYPE_BF16 = 0, 1
 
 
 class InvalidArgument(ValueError):
@@ -48,8 +49,13 @@ class _KvF8(C.Structure):
                 ("q_k", C.c_void_p), ("s_k", C.c_void_p), ("q_v", C.c_void_p), ("s_v", C.c_void_p)]
 
 
+class _KvB8(C.Structure):
+    _fields_ = [("H", C.c_int), ("D", C.c_int), ("page", C.c_int), ("npages", C.c_int), ("q_k", C.c_void_p),
+                ("s_k", C.c_void_p), ("q_v", C.c_void_p), ("s_v", C.c_void_p)]
+
+
 # Every symbol include/w4b_abi.h declares: name -> (restype, argtypes)
-_P, _I = C.c_void_p, C.c_int
+_P, _I, _L = C.c_void_p, C.c_int, C.c_longlong
 ABI = {
     "w4b_last_error": (C.c_char_p, []),
     "w4b_dispatch_mma_min_m": (_I, []),
@@ -83,6 +89,11 @@ ABI = {
     "w4b_attn_flash_w4_paged_batched": (_I, [C.POINTER(_KvW4), _P, _I, _P, _I, _I, _I, _I, _P, _P, _P]),
     "w4b_attn_single_fp16": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
     "w4b_attn_single_w4": (_I, [C.POINTER(_KvW4), _P, _P, _P, _P, _P]),
+    "w4b_page_tables": (_I, [_P, _P, _I, _I, _I, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _P]),
+    "w4b_kv_write_b8": (_I, [C.POINTER(_KvB8), _P, _I, _P, _P, _L, _L, _I, _P]),
+    "w4b_attn_b8_workspace": (_L, []),
+    "w4b_attn_b8_paged": (_I, [C.POINTER(_KvB8), _P, _I, _P, _P, _I, _I, _I, _P, _L, _I, _I, C.c_float, _I, _P, _L, _P,
+                               _P, _L, _P]),
     "w4b_peer_alloc": (_I, [C.c_size_t, C.POINTER(_P), _P]),
     "w4b_peer_open": (_I, [_P, C.POINTER(_P)]),
     "w4b_peer_close": (_I, [_P]),
@@ -182,6 +193,22 @@ class DeviceKVF8:  # include/w4/kvflash.cuh:390-396
 
     def _c(self):
         return _KvF8(self.H, self.S, self.D, self.gs, self.G, self.q_k, self.s_k, self.q_v, self.s_v)
+
+
+@dataclass
+class DeviceKVB8:
+    """Paged 8-bit cache: E4M3 codes [H][npages*page][D], FP32 scales [H][npages] (no reference counterpart)."""
+    H: int
+    D: int
+    page: int
+    npages: int
+    q_k: int
+    s_k: int
+    q_v: int
+    s_v: int
+
+    def _c(self):
+        return _KvB8(self.H, self.D, self.page, self.npages, self.q_k, self.s_k, self.q_v, self.s_v)
 
 
 # ---- entry points, named as in the reference ------------------------------
@@ -298,6 +325,43 @@ def kv_append_w4(p: DeviceKVW4, row, slab_rows, k_new, v_new, f16=False, stream=
 
 def kv_append_f8(p: DeviceKVF8, row, k_new, v_new, f16=False, stream=None):
     _check(lib.w4b_kv_append_f8(C.byref(p._c()), row, k_new, v_new, int(f16), stream))
+
+
+# ---- paged 8-bit cache: block tables, write, attention (no counterpart in the reference) --------
+
+def page_tables(cached, fresh, nseq, page, npages, free_pages, nfree, taken_in, taken_out, bt, bt_stride, seq_lens,
+                q_offsets, slots, positions, max_tokens, stream=None):
+    """Block tables, lengths, token offsets and the slot / position of every token of a step, from the requests'
+    cached[i] positions and fresh[i] new tokens. All arrays are device int32; new pages come from
+    free_pages[taken_in[0]:]. seq_lens may be cached and taken_out taken_in."""
+    _check(lib.w4b_page_tables(cached, fresh, nseq, page, npages, free_pages, nfree, taken_in, taken_out, bt, bt_stride,
+                               seq_lens, q_offsets, slots, positions, max_tokens, stream))
+
+
+def kv_write_b8(p: DeviceKVB8, slots, T, k_new, v_new, k_stride, v_stride, dtype=DTYPE_F16, stream=None):
+    """Quantises T tokens' keys and values (H*D FP16 / BF16 values every k_stride / v_stride values) into the rows
+    slots[t] of the cache; pages get or raise their scale as needed. slots[t] == -1 skips a token."""
+    _check(lib.w4b_kv_write_b8(C.byref(p._c()), slots, T, k_new, v_new, k_stride, v_stride, dtype, stream))
+
+
+def attention_b8_workspace() -> int:
+    """Bytes of a workspace of attention_b8_paged on the current device."""
+    n = lib.w4b_attn_b8_workspace()
+    if n < 0:
+        raise CudaError(lib.w4b_last_error().decode())
+    return n
+
+
+def attention_b8_paged(p: DeviceKVB8, bt, bt_stride, seq_lens, q_offsets, nseq, max_q, max_seq_len, q, q_stride, Hq,
+                       dtype, out, out_stride, lse=None, scale=None, causal=True, workspace=None, workspace_bytes=0,
+                       stream=None):
+    """Attention of the new tokens of nseq sequences over the paged 8-bit cache. q_offsets[i] .. q_offsets[i+1] are
+    sequence i's query tokens (None: one each); causal: they are its last positions; otherwise every token sees all
+    seq_lens[i] positions (cross attention). scale defaults to D ** -0.5. Calls that may overlap, captured ones
+    among them, need a zero-filled workspace each; without one they share library scratch."""
+    _check(lib.w4b_attn_b8_paged(C.byref(p._c()), bt, bt_stride, seq_lens, q_offsets, nseq, max_q, max_seq_len, q,
+                                 q_stride, Hq, dtype, max(p.D, 1) ** -0.5 if scale is None else scale, int(causal), out,
+                                 out_stride, lse, workspace, workspace_bytes, stream))
 
 
 # ---- offline re-layout: the same matrix zero-extended along K (no counterpart in the reference) ----

@@ -81,6 +81,7 @@ struct DeviceCtx {
   Scratch attn_ws;        // (m, l, acc[D]) partials of split sequences
   Scratch io_x, io_c;     // device staging of the host-buffer entry
   Scratch gemm_xpad;      // zero-padded activation rows of the padded-K entries
+  Scratch b8_ws;          // counters and partial results of the 8-bit paged attention: one size, never replaced
 };
 
 constexpr int kMaxDevices = 64;
@@ -707,6 +708,131 @@ int w4b_attn_flash_w4_paged_batched(const w4b_kv_w4* p, const int* bt, int bt_st
   CUDA_TRY(attn_flash_batched_launch(s, (const __half*)q, (__half*)out, p->H, p->D, nseq, seq_lens, bt_stride, max_splits,
                                      ctx->sm_count, (float*)ctx->attn_ws.ptr, (cudaStream_t)stream, &launches),
            "kv paged batched");
+  g_launches += (unsigned long long)launches;
+  return W4B_OK;
+}
+
+// ---- paged 8-bit cache: tables, write, attention (no counterpart in the reference) ------------
+
+int w4b_page_tables(const int* cached, const int* fresh, int nseq, int page, int npages, const int* free_pages, int nfree,
+                    const int* taken_in, int* taken_out, int* bt, int bt_stride, int* seq_lens, int* q_offsets, int* slots,
+                    int* positions, int max_tokens, void* stream) {
+  if (nseq < 1 || nseq > kMaxTableRequests) INVALID("page tables: nseq must be 1..%d", kMaxTableRequests);
+  if (page < 1 || npages < 1 || bt_stride < 1) INVALID("page tables: bad page geometry");
+  if ((long long)npages * page >= (1LL << 31)) INVALID("page tables: pool rows exceed 2^31");
+  if (nfree < 0 || max_tokens < 0) INVALID("page tables: negative count");
+  if (!cached || !fresh || !taken_in || !taken_out || !bt || !seq_lens || !q_offsets) INVALID("page tables: null pointer");
+  if (nfree > 0 && !free_pages) INVALID("page tables: null free list");
+  if (max_tokens > 0 && (!slots || !positions)) INVALID("page tables: null slot map");
+  DeviceCtx* ctx = nullptr;
+  if (int rc = get_ctx(&ctx)) return rc;
+  const PageTables a = {cached,    fresh, nseq,      page,  npages,    free_pages, nfree,       taken_in, taken_out,
+                        bt, bt_stride, seq_lens, q_offsets, slots, positions, max_tokens, ctx->status};
+  CUDA_TRY(page_tables_launch(a, (cudaStream_t)stream), "page tables kernel");
+  g_launches += 1;
+  return W4B_OK;
+}
+
+namespace {
+int check_kv_b8(const w4b_kv_b8* p, const char* who) {
+  if (!p) INVALID("%s: null descriptor", who);
+  if (p->H < 1 || p->page < 1 || p->npages < 1) INVALID("%s: bad dims", who);
+  if (p->H > 65535) INVALID("%s: more than 65535 heads", who);
+  if (p->D != 64 && p->D != 128) INVALID("%s: D must be 64 or 128", who);
+  if (p->page % 16 != 0 || p->page > 4096) INVALID("%s: page must be a multiple of 16, at most 4096", who);
+  if ((long long)p->npages * p->page >= (1LL << 31)) INVALID("%s: pool rows exceed 2^31", who);
+  if (!p->q_k || !p->s_k || !p->q_v || !p->s_v) INVALID("%s: null pointer", who);
+  if (((uintptr_t)p->q_k | (uintptr_t)p->q_v) & 15u) INVALID("%s: cache bases must be 16-byte aligned", who);
+  if (((uintptr_t)p->s_k | (uintptr_t)p->s_v) & 3u) INVALID("%s: scales must be 4-byte aligned", who);
+  return W4B_OK;
+}
+int check_rows(const void* p, long long stride, long long width, const char* what, const char* who) {
+  if (!p) INVALID("%s: null %s", who, what);
+  if (((uintptr_t)p & 15u) || stride % 8 != 0) INVALID("%s: %s rows must be 16-byte aligned", who, what);
+  if (stride < width) INVALID("%s: %s rows overlap", who, what);
+  return W4B_OK;
+}
+}  // namespace
+
+int w4b_kv_write_b8(const w4b_kv_b8* p, const int* slots, int T, const void* k_new, const void* v_new, long long k_stride,
+                    long long v_stride, int dtype, void* stream) {
+  const char* who = "kv write b8";
+  if (int rc = check_kv_b8(p, who)) return rc;
+  if (T < 0) INVALID("%s: negative token count", who);
+  if (dtype != W4B_DTYPE_F16 && dtype != W4B_DTYPE_BF16) INVALID("%s: unknown dtype %d", who, dtype);
+  if (!slots) INVALID("%s: null slot map", who);
+  if (int rc = check_rows(k_new, k_stride, (long long)p->H * p->D, "key", who)) return rc;
+  if (int rc = check_rows(v_new, v_stride, (long long)p->H * p->D, "value", who)) return rc;
+  if (T == 0) return W4B_OK;
+  DeviceCtx* ctx = nullptr;
+  if (int rc = get_ctx(&ctx)) return rc;
+  const KvWriteB8 a = {slots, T, k_new, v_new, k_stride, v_stride, p->page, p->npages, p->q_k, p->s_k, p->q_v, p->s_v, 1, ctx->status};
+  CUDA_TRY(kv_write_b8_launch(a, p->H, p->D, dtype == W4B_DTYPE_BF16, ctx->sm_count, (cudaStream_t)stream), "kv write b8 kernel");
+  g_launches += 1;
+  return W4B_OK;
+}
+
+long long w4b_attn_b8_workspace(void) {
+  DeviceCtx* ctx = nullptr;
+  if (get_ctx(&ctx)) return -1;
+  return (long long)attn_b8_ws_bytes(ctx->sm_count);
+}
+
+int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const int* seq_lens, const int* q_offsets, int nseq,
+                      int max_q, int max_seq_len, const void* q, long long q_stride, int Hq, int dtype, float scale,
+                      int causal, void* out, long long out_stride, float* lse, void* ws, long long ws_bytes, void* stream) {
+  const char* who = "attention b8";
+  if (int rc = check_kv_b8(p, who)) return rc;
+  if (nseq < 1 || max_q < 1 || max_seq_len < 0) INVALID("%s: bad sequence count or length", who);
+  if (Hq < 1 || Hq % p->H != 0) INVALID("%s: query heads must be a multiple of the cache's heads", who);
+  if (dtype != W4B_DTYPE_F16 && dtype != W4B_DTYPE_BF16) INVALID("%s: unknown dtype %d", who, dtype);
+  if (!(scale > 0.0f && scale < 1e30f)) INVALID("%s: scale must be positive", who);
+  if (!bt || !seq_lens) INVALID("%s: null pointer", who);
+  if (!q_offsets && max_q != 1) INVALID("%s: without q_offsets every sequence has one query token", who);
+  if (max_seq_len > 65535 * kFlashTile) INVALID("%s: sequence exceeds the tile-grid bound", who);
+  if (bt_stride < (max_seq_len + p->page - 1) / p->page) INVALID("%s: block-table rows shorter than the longest sequence", who);
+  if ((long long)max_q * (Hq / p->H) > INT_MAX / 2) INVALID("%s: too many query rows", who);
+  if (int rc = check_rows(q, q_stride, (long long)Hq * p->D, "query", who)) return rc;
+  if (int rc = check_rows(out, out_stride, (long long)Hq * p->D, "output", who)) return rc;
+  if (lse && ((uintptr_t)lse & 3u)) INVALID("%s: lse must be 4-byte aligned", who);
+  if (ws && ((uintptr_t)ws & 255u)) INVALID("%s: the workspace must be 256-byte aligned", who);
+  DeviceCtx* ctx = nullptr;
+  if (int rc = get_ctx(&ctx)) return rc;
+  const size_t need = attn_b8_ws_bytes(ctx->sm_count);
+  if (ws) {
+    if (ws_bytes < (long long)need) INVALID("%s: workspace of %lld bytes, %zu are needed", who, ws_bytes, need);
+  } else {
+    CUDA_TRY(ctx->b8_ws.reserve(need, true), "attention workspace");
+    ws = ctx->b8_ws.ptr;
+  }
+  AttnB8 a;
+  memset(&a, 0, sizeof(a));
+  a.q_k = p->q_k;
+  a.s_k = p->s_k;
+  a.q_v = p->q_v;
+  a.s_v = p->s_v;
+  a.H = p->H;
+  a.page = p->page;
+  a.npages = p->npages;
+  a.bt = bt;
+  a.bt_stride = bt_stride;
+  a.seq_lens = seq_lens;
+  a.q_offsets = q_offsets;
+  a.nseq = nseq;
+  a.max_q = max_q;
+  a.max_len = max_seq_len;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.group = Hq / p->H;
+  a.scale = scale;
+  a.causal = causal ? 1 : 0;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.lse = lse;
+  a.ws = ws;
+  a.status = ctx->status;
+  int launches = 0;
+  CUDA_TRY(attn_b8_launch(a, p->D, dtype == W4B_DTYPE_BF16, ctx->sm_count, (cudaStream_t)stream, &launches), who);
   g_launches += (unsigned long long)launches;
   return W4B_OK;
 }

@@ -1,0 +1,584 @@
+// Attention over a paged 8-bit cache (E4M3 codes, one FP32 scale per page and key/value head), for a few query tokens
+// per sequence: decode steps, drafted tokens, and the same without the causal mask over an encoder's states.
+//
+// Mathematics, per sequence and key/value head. The R = tokens * group query rows that share the head are columns of
+//   X[pos][n] = (K q)[pos][n] * (s_k * scale * log2 e) + log2(s_v)         x = log2 of the weight of the CODE row of V
+//   w = 2^(X - m),  O^T[d][n] += sum_pos Vcode[pos][d] * w[pos][n],  l[n] += w / s_v
+// with m a reference point near the running maximum of X: taking log2(s_v) into the exponent puts V's scale into the
+// weights for free, whatever its size, and w / s_v is the plain softmax weight. out = O / l, lse = ln 2 (m + log2 l).
+// m moves only when some X exceeds it by more than 8 (a warp vote), so the usual block needs no reduction across
+// lanes: weights up to 2^8 are exact-enough halves, sums are FP32.
+//
+// Both products run on mma.sync.m16n8k16 with the CACHE as the 16-row operand and the query rows as the 8 columns
+// (a decode step has 1 to 16 rows: as the 128-row operand of the larger tensor instructions they would leave most of
+// it empty, and at HBM speed this form needs a sixth of the mma.sync rate):
+//   K: ldmatrix hands lane (g, c) bytes 4c..4c+3 of a 16-byte piece of positions g and g + 8; two conversions
+//      E4M3x2 -> half2 make them the operand's registers (the k order is permuted, q is loaded in the same order);
+//   V: ldmatrix.trans hands over dims 2g, 2g+1 of positions 2c, 2c+1; one byte permute pairs the positions, two
+//      conversions make the transposed operand (row g = dim 2g, row g + 8 = dim 2g + 1).
+// E4M3 -> FP16 is exact. The weights go from accumulator to operand layout by movmatrix.
+//
+// Bound by HBM: the cache is read once. Each warp keeps its own ring of 16-position blocks (K and V, 4 KB at D = 128)
+// filled by cp.async three blocks ahead, without any barrier between warps.
+//
+// Split: all work - 64-position units of all (sequence, head, column tile) rows in order - is cut into equal ranges,
+// one per CTA, whatever the lengths; the lengths are on the device, so every CTA sums them itself. A row that spans
+// CTAs is joined by whichever of them arrives last, in CTA order (bit-identical from run to run).
+#include <cuda_bf16.h>
+#include <float.h>
+
+#include "w4b_common.cuh"
+#include "w4b_kernels.h"
+
+namespace w4b {
+namespace {
+
+constexpr int AB_WARPS = 4;
+constexpr int AB_THREADS = 32 * AB_WARPS;
+constexpr int AB_CTAS_PER_SM = 4;
+constexpr int AB_STAGES = 3;
+constexpr int AB_UNIT = 64;      // positions per work unit: one block of 16 per warp
+constexpr int AB_MAX_COLS = 16;  // query rows per column tile
+constexpr int AB_MAX_D = 128;
+constexpr float AB_LOG2E = 1.4426950408889634f;
+constexpr float AB_LN2 = 0.6931471805599453f;
+constexpr float AB_SLACK = 8.0f;   // how far a weight's exponent may exceed the reference point
+constexpr float AB_NONE = -1e30f;  // reference point of a column that has seen nothing
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// bytes 0, 1 (lo) and 2, 3 (hi) of w to half2 each
+__device__ __forceinline__ void e4m3x4_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n"
+      ".reg .b16 a, b;\n"
+      "mov.b32 {a, b}, %2;\n"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n"
+      "}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a sequence asks for, with the device-side values held inside what the launch was sized for.
+struct SeqInfo {
+  int len, q0, nq;
+};
+__device__ __forceinline__ SeqInfo seq_info(const AttnB8& a, int i) {
+  SeqInfo s;
+  s.len = min(max(a.seq_lens[i], 0), a.max_len);
+  s.q0 = a.q_offsets ? a.q_offsets[i] : i;
+  s.nq = a.q_offsets ? min(max(a.q_offsets[i + 1] - s.q0, 0), a.max_q) : 1;
+  return s;
+}
+
+template <int NC>
+__device__ __forceinline__ long long seq_units(const AttnB8& a, const SeqInfo& s, int& tiles, int& units) {
+  tiles = (s.nq * a.group + NC - 1) / NC;
+  units = max(1, (s.len + AB_UNIT - 1) / AB_UNIT);
+  return (long long)a.H * tiles * units;
+}
+
+template <typename T>
+__device__ __forceinline__ T block_exclusive(T v, T* sums, T& total) {  // AB_THREADS threads
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  T x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const T o = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += o;
+  }
+  if (lane == 31) sums[wid] = x;
+  __syncthreads();
+  T before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < AB_WARPS; ++w) {
+    if (w < wid) before += sums[w];
+    total += sums[w];
+  }
+  __syncthreads();
+  return before + x - v;
+}
+
+template <int D, int NT, bool BF16>
+struct AttnB8Kernel {
+  static constexpr int NC = 8 * NT;
+  static constexpr int KSTEPS = D / 16;             // MMAs per 16 positions and column octet, each product
+  static constexpr int PIECES = D / 16;             // 16-byte pieces per row
+  static constexpr int SIDE = 16 * D;               // bytes of K (or V) in a block
+  static constexpr int STAGE = 2 * SIDE + 16;       // + s_k, s_v
+  static constexpr int RING = AB_STAGES * STAGE;    // per warp
+  static constexpr int OPITCH = D + 8;              // floats per column of the merge buffer
+  static constexpr int MERGE = AB_WARPS * NC * (OPITCH + 2) * 4;
+  static constexpr int SMEM = (AB_WARPS * RING > MERGE ? AB_WARPS * RING : MERGE);
+  static constexpr size_t PART = (size_t)NC * (D + 2);  // floats of a partial result
+
+  // 16-byte piece j of row r of a block, swizzled so that eight rows of one piece meet all banks
+  static __device__ __forceinline__ uint32_t piece(int r, int j) {
+    if (D == 128) return (uint32_t)(r * 128 + ((j ^ (r & 7)) << 4));
+    return (uint32_t)(r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+  }
+};
+
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(const AttnB8 a) {
+  using C = AttnB8Kernel<D, NT, BF16>;
+  constexpr int NC = C::NC;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long sums[AB_WARPS];
+  __shared__ long long found_off;
+  __shared__ int found_seq, is_last;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
+
+  // ---- this CTA's range of units -----------------------------------------------------------------------------
+  const int per = (a.nseq + AB_THREADS - 1) / AB_THREADS;
+  const int i_begin = min(tid * per, a.nseq), i_end = min(i_begin + per, a.nseq);
+  long long mine = 0;
+  int tiles, units;
+  for (int i = i_begin; i < i_end; ++i) mine += seq_units<NC>(a, seq_info(a, i), tiles, units);
+  long long T;
+  const long long before = block_exclusive(mine, sums, T);
+  const long long G = T < (long long)gridDim.x ? T : (long long)gridDim.x;
+  const long long cta = blockIdx.x;
+  if (cta >= G) return;
+  const long long u_begin = T * cta / G, u_end = T * (cta + 1) / G;
+  if (u_begin >= before && u_begin < before + mine) {
+    long long off = u_begin - before;
+    int i = i_begin;
+    for (;; ++i) {
+      const long long n = seq_units<NC>(a, seq_info(a, i), tiles, units);
+      if (off < n) break;
+      off -= n;
+    }
+    found_seq = i;
+    found_off = off;
+  }
+  __syncthreads();
+  int seq = found_seq;
+  long long off = found_off;  // units into the sequence
+  long long u = u_begin;
+
+  int* counters = (int*)a.ws;
+  float* parts = (float*)((uint8_t*)a.ws + 4 * (((size_t)gridDim.x + 63) / 64 * 64));
+  const uint32_t ring = smem_u32(smem) + wid * C::RING;
+
+  while (u < u_end) {
+    const SeqInfo s = seq_info(a, seq);
+    const long long seq_n = seq_units<NC>(a, s, tiles, units);
+    if (off >= seq_n) {
+      ++seq;
+      off = 0;
+      continue;
+    }
+    // row = (head, column tile) of the sequence; units [r0, r1) of it are this CTA's
+    const int row = (int)(off / units), r0 = (int)(off - (long long)row * units);
+    const int r1 = (int)min((long long)units, r0 + (u_end - u));
+    const int head = row / tiles, tile = row - head * tiles;
+    const int rows = min(NC, s.nq * a.group - tile * NC);   // query rows in this tile
+    const int tq0 = tile * NC / a.group;                      // first and last query token of the tile
+    const int tq1 = (tile * NC + rows - 1) / a.group;
+    const int end = a.causal ? min(s.len, max(0, s.len - s.nq + tq1 + 1)) : s.len;  // positions any row sees
+    const int all_see = a.causal ? max(0, s.len - s.nq + tq0 + 1) : s.len;          // positions every row sees
+    const int p_begin = r0 * AB_UNIT, p_end = min(r1 * AB_UNIT, end);
+    const int nblocks = p_end > p_begin ? (p_end - p_begin + 15) / 16 : 0;
+    const int mine_n = nblocks > wid ? (nblocks - wid + AB_WARPS - 1) / AB_WARPS : 0;
+
+    // ---- query rows as operand registers: lane (g, c) holds row g, dims 16 i + 4 c .. + 3 ----------------------
+    uint32_t qf[NT][C::KSTEPS][2];
+    float fs[NT][2];     // per column (2c, 2c + 1): score factor without s_k
+    int lim[NT][2];      // per column: positions it sees
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = t * 8 + g, r = tile * NC + n;
+      const bool on = n < rows;
+      const int tq = on ? r / a.group : 0, hh = on ? r - tq * a.group : 0;
+      const uint16_t* qrow =
+          (const uint16_t*)a.q + (long long)(s.q0 + tq) * a.q_stride + (size_t)(head * a.group + hh) * D + 4 * c;
+      float scale_row = 1.0f;
+      if (!BF16) {
+#pragma unroll
+        for (int i = 0; i < C::KSTEPS; ++i) {
+          const uint2 v = on ? *(const uint2*)(qrow + 16 * i) : make_uint2(0, 0);
+          qf[t][i][0] = v.x;
+          qf[t][i][1] = v.y;
+        }
+      } else {
+        // BF16 to FP16 by a power of two of the row's own: its largest value lands in [2^14, 2^15), what falls
+        // below the half range is 2^-39 of it
+        uint2 v[C::KSTEPS];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < C::KSTEPS; ++i) {
+          v[i] = on ? *(const uint2*)(qrow + 16 * i) : make_uint2(0, 0);
+          top = __vmaxu2(top, __vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu));
+        }
+        top = max(top & 0xFFFFu, top >> 16);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (int)(top >> 7);  // biased exponent
+        const int k = min(max(141 - e, -100), 100);  // 127 + 14 - e
+        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
+        scale_row = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+        for (int i = 0; i < C::KSTEPS; ++i) {
+          const uint32_t w[2] = {v[i].x, v[i].y};
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            qf[t][i][j] = h2_as_u32(__floats2half2_rn(__uint_as_float(w[j] << 16) * up,
+                                                      __uint_as_float(w[j] & 0xFFFF0000u) * up));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int col = 2 * c + j;
+        fs[t][j] = __shfl_sync(0xffffffffu, scale_row, col * 4) * (a.scale * AB_LOG2E);
+        const int rr = tile * NC + t * 8 + col;
+        lim[t][j] = t * 8 + col < rows ? (a.causal ? s.len - s.nq + rr / a.group + 1 : s.len) : 0;
+      }
+    }
+
+    float acc[C::KSTEPS][NT][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int i = 0; i < C::KSTEPS; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][t][j] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[t][j] = AB_NONE;
+        l[t][j] = 0.0f;
+      }
+
+    // ---- the ring ------------------------------------------------------------------------------------------------
+    const int* bt = a.bt + (long long)seq * a.bt_stride;
+    const size_t slab = (size_t)head * a.npages;
+    auto position = [&](int j) { return p_begin + (wid + j * AB_WARPS) * 16; };
+    auto page_of = [&](int j) { return j < mine_n ? bt[position(j) / a.page] : 0; };
+    auto issue = [&](int j, int pg) {
+      const uint32_t st = ring + (j % AB_STAGES) * C::STAGE;
+      if (j < mine_n) {
+        const int p0 = position(j);
+        const bool good = (unsigned)pg < (unsigned)a.npages;
+        const size_t r = (slab + (good ? pg : 0)) * a.page + (p0 - p0 / a.page * a.page);
+        const uint8_t* ks = a.q_k + r * D;
+        const uint8_t* vs = a.q_v + r * D;
+#pragma unroll
+        for (int i = 0; i < C::SIDE / 512; ++i) {
+          const int e = i * 32 + lane, rr = e / C::PIECES, jj = e - rr * C::PIECES;
+          const bool on = good && p0 + rr < s.len;
+          cp_async16_zfill(st + C::piece(rr, jj), ks + (on ? e * 16 : 0), on);
+          cp_async16_zfill(st + C::SIDE + C::piece(rr, jj), vs + (on ? e * 16 : 0), on);
+        }
+        if (lane < 2) {
+          const float* sc = (lane == 0 ? a.s_k : a.s_v) + slab + (good ? pg : 0);
+          if (good) {
+            cp_async<4>(st + 2 * C::SIDE + 4 * lane, sc);
+          } else {
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * C::SIDE + 4 * lane), "f"(-1.0f) : "memory");
+            if (lane == 0) atomicExch(a.status, ST_KV_PAGE);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    int pg_next = page_of(0);
+#pragma unroll
+    for (int j = 0; j < AB_STAGES - 1; ++j) {
+      const int pg = pg_next;
+      pg_next = page_of(j + 1);
+      issue(j, pg);
+    }
+
+    for (int j = 0; j < mine_n; ++j) {
+      cp_async_wait<AB_STAGES - 2>();
+      __syncwarp();
+      {
+        const int pg = pg_next;
+        pg_next = page_of(j + AB_STAGES);
+        issue(j + AB_STAGES - 1, pg);
+      }
+      const uint32_t st = ring + (j % AB_STAGES) * C::STAGE;
+      const int p0 = position(j);
+      const float sk = __uint_as_float(lds32(st + 2 * C::SIDE)), sv = __uint_as_float(lds32(st + 2 * C::SIDE + 4));
+      // scores
+      float x[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[t][i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < C::KSTEPS; i += 2) {
+        uint32_t r[4];
+        // matrices: positions 0-7 and 8-15 of piece i, then of piece i + 1
+        ldsm4(r, st + C::piece((lane & 7) + (lane & 8), i + (lane >> 4)));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t f[4];
+          e4m3x4_to_h2(r[2 * k], f[0], f[2]);
+          e4m3x4_to_h2(r[2 * k + 1], f[1], f[3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_16816(x[t], f, qf[t][i + k][0], qf[t][i + k][1]);
+        }
+      }
+      // weights
+      const bool bad = sv < 0.0f;
+      const float svc = fmaxf(sv, 1e-30f), lv = lg2(svc), inv_sv = __frcp_rn(svc);
+      const bool partial = bad || p0 + 16 > all_see;
+      bool over = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[t][i] = fmaf(x[t][i], fs[t][i & 1] * sk, lv);
+          if (partial && (bad || p0 + g + (i >> 1) * 8 >= lim[t][i & 1])) x[t][i] = -INFINITY;
+          over = over || x[t][i] > m[t][i & 1] + AB_SLACK;
+        }
+      }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(x[t][i], x[t][i + 2]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            // (only the columns that need it: a column's bits do not depend on the others')
+            const float mn = top > m[t][i] + AB_SLACK ? top : m[t][i], f = ex2(m[t][i] - mn);
+            m[t][i] = mn;
+            l[t][i] *= f;
+#pragma unroll
+            for (int k = 0; k < C::KSTEPS; ++k) {
+              acc[k][t][i] *= f;
+              acc[k][t][i + 2] *= f;
+            }
+          }
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = ex2(x[t][i] - m[t][i & 1]);
+          l[t][i & 1] = fmaf(w[i], inv_sv, l[t][i & 1]);
+        }
+        // rounded to halves: 2^-12 of a weight at most on average over many positions, as exact as the FP16 output
+        pf[t][0] = movmatrix_trans(h2_as_u32(__floats2half2_rn(w[0], w[1])));
+        pf[t][1] = movmatrix_trans(h2_as_u32(__floats2half2_rn(w[2], w[3])));
+      }
+      // values
+#pragma unroll
+      for (int i = 0; i < C::KSTEPS; i += 2) {
+        uint32_t r[4];
+        ldsm4_trans(r, st + C::SIDE + C::piece((lane & 7) + (lane & 8), i + (lane >> 4)));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t f[4];
+          e4m3x4_to_h2(__byte_perm(r[2 * k], 0, 0x3120), f[0], f[1]);
+          e4m3x4_to_h2(__byte_perm(r[2 * k + 1], 0, 0x3120), f[2], f[3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_16816(acc[i + k][t], f, pf[t][0], pf[t][1]);
+        }
+      }
+      __syncwarp();
+    }
+
+    // ---- join the warps ------------------------------------------------------------------------------------------
+    cp_async_wait<0>();
+    __syncthreads();  // the ring becomes the merge buffer
+    float* om = (float*)smem;                           // [warp][NC][OPITCH]
+    float* ml = om + AB_WARPS * NC * C::OPITCH;           // [warp][NC][2]
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = l[t][j];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int n = t * 8 + 2 * c + j;
+        if (g == 0) {
+          ml[(wid * NC + n) * 2] = m[t][j];
+          ml[(wid * NC + n) * 2 + 1] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < C::KSTEPS; ++i)
+          *(float2*)(om + (wid * NC + n) * C::OPITCH + 16 * i + 2 * g) = make_float2(acc[i][t][j], acc[i][t][j + 2]);
+      }
+    __syncthreads();
+
+    // where the row begins and ends among the CTAs
+    const long long row_begin = u - r0, row_end = row_begin + units;
+    const bool whole = r0 == 0 && r1 == units;
+    const int first_cta = (int)(((row_begin + 1) * G - 1) / T), last_cta = (int)((row_end * G - 1) / T);
+    constexpr int LANES = D / 8;  // threads per column
+    auto store_row = [&](int n, int d, const float v[8], float ms, float ls) {
+      // d: first of eight dims; v unnormalised
+      const int r = tile * NC + n, tq = r / a.group, hq = head * a.group + (r - tq * a.group);
+      const float inv = ls > 0.0f ? 1.0f / ls : (ls == 0.0f ? 0.0f : ls);  // nothing seen: zeros; NaN stays
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = v[2 * i] * inv, q = v[2 * i + 1] * inv;
+        if (BF16) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(p, q);
+          h[i] = *(const uint32_t*)&b;
+        } else {
+          h[i] = h2_as_u32(__floats2half2_rn(p, q));
+        }
+      }
+      *(uint4*)((uint16_t*)a.out + (long long)(s.q0 + tq) * a.out_stride + (size_t)hq * D + d) =
+          make_uint4(h[0], h[1], h[2], h[3]);
+      if (a.lse && d == 0)
+        a.lse[(long long)(s.q0 + tq) * (a.H * a.group) + hq] = ls == 0.0f ? -INFINITY : (ms + log2f(ls)) * AB_LN2;
+    };
+    float* part = parts + (size_t)(2 * cta + (r0 == 0 ? 1 : 0)) * C::PART;
+    for (int e = tid; e < NC * LANES; e += AB_THREADS) {
+      const int n = e / LANES, d = (e - n * LANES) * 8;
+      if (n >= rows) continue;
+      float ms = AB_NONE, ls = 0.0f, v[8];
+#pragma unroll
+      for (int w = 0; w < AB_WARPS; ++w) ms = fmaxf(ms, ml[(w * NC + n) * 2]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < AB_WARPS; ++w) {
+        const float f = ex2(ml[(w * NC + n) * 2] - ms);
+        ls = fmaf(ml[(w * NC + n) * 2 + 1], f, ls);
+        const float4* o = (const float4*)(om + (w * NC + n) * C::OPITCH + d);
+        const float4 o0 = o[0], o1 = o[1];
+        v[0] = fmaf(o0.x, f, v[0]);
+        v[1] = fmaf(o0.y, f, v[1]);
+        v[2] = fmaf(o0.z, f, v[2]);
+        v[3] = fmaf(o0.w, f, v[3]);
+        v[4] = fmaf(o1.x, f, v[4]);
+        v[5] = fmaf(o1.y, f, v[5]);
+        v[6] = fmaf(o1.z, f, v[6]);
+        v[7] = fmaf(o1.w, f, v[7]);
+      }
+      if (whole) {
+        store_row(n, d, v, ms, ls);
+      } else {
+        float4* dst = (float4*)(part + 2 * NC + n * D + d);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+        if (d == 0) *(float2*)(part + 2 * n) = make_float2(ms, ls);
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const int want = last_cta - first_cta + 1;
+        const int got = atomicAdd(counters + first_cta, 1) + 1;
+        is_last = got == want;
+        if (got == want) counters[first_cta] = 0;  // as the next launch expects it
+      }
+      __syncthreads();
+      if (is_last) {
+        __threadfence();
+        for (int e = tid; e < NC * LANES; e += AB_THREADS) {
+          const int n = e / LANES, d = (e - n * LANES) * 8;
+          if (n >= rows) continue;
+          auto slot = [&](int k) { return parts + (size_t)(k == first_cta ? 2 * k + 1 : 2 * k) * C::PART; };
+          float ms = AB_NONE, ls = 0.0f, v[8];
+          for (int k = first_cta; k <= last_cta; ++k) ms = fmaxf(ms, __ldcg(slot(k) + 2 * n));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+#pragma unroll 4
+          for (int k = first_cta; k <= last_cta; ++k) {
+            const float* src = slot(k);
+            const float2 st = __ldcg((const float2*)(src + 2 * n));
+            const float4 o0 = __ldcg((const float4*)(src + 2 * NC + n * D + d));
+            const float4 o1 = __ldcg((const float4*)(src + 2 * NC + n * D + d) + 1);
+            const float f = ex2(st.x - ms);
+            ls = fmaf(st.y, f, ls);
+            v[0] = fmaf(o0.x, f, v[0]);
+            v[1] = fmaf(o0.y, f, v[1]);
+            v[2] = fmaf(o0.z, f, v[2]);
+            v[3] = fmaf(o0.w, f, v[3]);
+            v[4] = fmaf(o1.x, f, v[4]);
+            v[5] = fmaf(o1.y, f, v[5]);
+            v[6] = fmaf(o1.z, f, v[6]);
+            v[7] = fmaf(o1.w, f, v[7]);
+          }
+          store_row(n, d, v, ms, ls);
+        }
+      }
+    }
+    __syncthreads();  // the merge buffer becomes the ring again
+    u += r1 - r0;
+    off += r1 - r0;
+  }
+}
+
+int attn_b8_grid(int sm_count) { return AB_CTAS_PER_SM * sm_count; }
+size_t counter_bytes(int grid) { return 4 * (((size_t)grid + 63) / 64 * 64); }
+
+template <int D, int NT, bool BF16>
+cudaError_t launch(const AttnB8& a, int sm_count, cudaStream_t stream) {
+  using C = AttnB8Kernel<D, NT, BF16>;
+  auto* k = attn_b8_kernel<D, NT, BF16>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return e;
+  k<<<attn_b8_grid(sm_count), AB_THREADS, C::SMEM, stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t attn_b8_ws_bytes(int sm_count) {
+  const int grid = attn_b8_grid(sm_count);
+  return counter_bytes(grid) + (size_t)2 * grid * AB_MAX_COLS * (AB_MAX_D + 2) * sizeof(float);
+}
+
+cudaError_t attn_b8_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaStream_t stream, int* launches) {
+  const bool wide = (long long)a.max_q * a.group > 8;
+  *launches = 1;
+#define W4B_GO(DD)                                                                                      \
+  (bf16 ? (wide ? launch<DD, 2, true>(a, sm_count, stream) : launch<DD, 1, true>(a, sm_count, stream)) \
+        : (wide ? launch<DD, 2, false>(a, sm_count, stream) : launch<DD, 1, false>(a, sm_count, stream)))
+  return D == 128 ? W4B_GO(128) : W4B_GO(64);
+#undef W4B_GO
+}
+
+}  // namespace w4b

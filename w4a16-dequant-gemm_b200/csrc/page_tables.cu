@@ -1,0 +1,188 @@
+// Block tables and slot maps of one serving step, from the requests' lengths, on the device.
+//
+// Request i holds cached[i] positions and brings fresh[i] new tokens. With P positions per page it needs
+//   need_i = ceil((cached_i + fresh_i) / P) - ceil(cached_i / P)
+// further pages; they are the entries [taken + sum_{j<i} need_j, ... + need_i) of the free list. Token t of the step
+// (requests in order, a request's tokens in order) has position cached_i + (t - q_offsets_i) and slot
+// bt[i][position / P] * P + position % P.
+//
+// A few kilobytes: bound by latency, so one launch does all of it. The grid is ONE cluster of up to eight CTAs. Every
+// CTA computes the two exclusive sums over all requests by itself (a few loads per thread) into shared memory; then
+// the cluster's threads share the requests, the new pages and the tokens, each finding its request by binary search
+// in the sums - balanced however unequal the requests are. The cluster barrier between the reads of `cached` /
+// `taken_in` and the first write lets the caller advance both in place.
+#include <limits.h>
+
+#include "w4b_common.cuh"
+#include "w4b_kernels.h"
+
+namespace w4b {
+namespace {
+
+constexpr int PT_THREADS = 1024;
+constexpr int PT_CLUSTER = 8;   // the portable cluster size
+constexpr int PT_TOKENS = 4;    // consecutive tokens per thread: one search, one 16-byte store per array
+
+__device__ __forceinline__ long long warp_inclusive(long long v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int clamp_int(long long v) { return v > INT_MAX ? INT_MAX : (int)v; }
+
+// The last i with off[i] <= v (off ascending, off[0] == 0 <= v).
+__device__ __forceinline__ int find_last(const int* off, int n, int v) {
+  int lo = 0, hi = n;  // off[lo] <= v; off[hi] > v or hi == n
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid] <= v) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(PT_THREADS, 1) page_tables_kernel(const PageTables a) {
+  extern __shared__ int sm[];
+  int* tok = sm;                  // exclusive sums of fresh, nseq + 1 values (saturated)
+  int* pg = tok + a.nseq + 1;     // exclusive sums of need
+  int* have = pg + a.nseq + 1;    // cached positions; -1: the request does not fit its table row
+  __shared__ long long wsum[2][PT_THREADS / 32], carry[2];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int taken = max(0, *a.taken_in);
+  if (tid < 2) carry[tid] = 0;
+  __syncthreads();
+
+  const long long room = (long long)min(a.bt_stride, a.npages) * a.page;
+  bool bad = false;
+  for (int i0 = 0; i0 < a.nseq; i0 += PT_THREADS) {
+    const int i = i0 + tid;
+    long long f = 0, need = 0;
+    if (i < a.nseq) {
+      const int c = a.cached[i], fr = a.fresh[i];
+      f = max(0, fr);
+      const bool fits = c >= 0 && fr >= 0 && (long long)c + fr <= room;
+      bad = bad || !fits;
+      if (fits) need = (c + fr + (long long)a.page - 1) / a.page - (c + (long long)a.page - 1) / a.page;
+      have[i] = fits ? c : -1;
+    }
+    const long long fi = warp_inclusive(f, lane), ni = warp_inclusive(need, lane);
+    if (lane == 31) {
+      wsum[0][wid] = fi;
+      wsum[1][wid] = ni;
+    }
+    __syncthreads();
+    if (wid < 2) {  // warp 0: tokens, warp 1: pages
+      const long long v = wsum[wid][lane], s = warp_inclusive(v, lane);
+      const long long before = carry[wid];
+      __syncwarp();
+      wsum[wid][lane] = before + s - v;
+      if (lane == 31) carry[wid] = before + s;
+    }
+    __syncthreads();
+    if (i < a.nseq) {
+      tok[i] = clamp_int(wsum[0][wid] + fi - f);
+      pg[i] = clamp_int(wsum[1][wid] + ni - need);
+    }
+    __syncthreads();
+  }
+  const long long total_tok = carry[0], total_pg = carry[1];
+  if (tid == 0) {
+    tok[a.nseq] = clamp_int(total_tok);
+    pg[a.nseq] = clamp_int(total_pg);
+  }
+  const int cta = (int)blockIdx.x;
+  if (bad && cta == 0) atomicExch(a.status, ST_PAGES_INVALID);
+  // every CTA has read cached and taken_in: from here on the outputs may overwrite them
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncthreads();
+
+  const int gt = cta * PT_THREADS + tid, gn = (int)gridDim.x * PT_THREADS;
+  const long long left = (long long)a.nfree - taken;  // pages still in the list
+  if (gt == 0) {
+    *a.taken_out = (int)(taken + (total_pg < left ? total_pg : (left > 0 ? left : 0)));
+    if (total_pg > left) atomicExch(a.status, ST_PAGES_EXHAUSTED);
+    else if (total_tok > a.max_tokens) atomicExch(a.status, ST_PAGES_INVALID);
+  }
+  for (int i = gt; i <= a.nseq; i += gn) {
+    a.q_offsets[i] = tok[i];
+    if (i < a.nseq) a.seq_lens[i] = have[i] < 0 ? 0 : have[i] + (tok[i + 1] - tok[i]);
+  }
+  // entry `at` of the free list, -1 behind its end or for a page the pool does not have
+  auto listed = [&](long long at) {
+    const int p = at < a.nfree ? a.free_pages[at] : -1;
+    return (unsigned)p < (unsigned)a.npages ? p : -1;
+  };
+  for (int j = gt; j < pg[a.nseq]; j += gn) {
+    const int i = find_last(pg, a.nseq, j);
+    const int col = (have[i] + a.page - 1) / a.page + (j - pg[i]);
+    a.bt[(long long)i * a.bt_stride + col] = listed((long long)taken + j);
+  }
+  const bool vec = ((((uintptr_t)a.slots | (uintptr_t)a.positions) & 15u) == 0);
+  for (long long t0 = (long long)gt * PT_TOKENS; t0 < a.max_tokens; t0 += (long long)gn * PT_TOKENS) {
+    int slot[PT_TOKENS], pos[PT_TOKENS];
+    int i = t0 < tok[a.nseq] ? find_last(tok, a.nseq, (int)t0) : 0;
+#pragma unroll
+    for (int k = 0; k < PT_TOKENS; ++k) {
+      const long long t = t0 + k;
+      slot[k] = -1;
+      pos[k] = 0;
+      if (t < tok[a.nseq]) {
+        while (tok[i + 1] <= t) ++i;  // ends: tok[nseq] > t
+        if (have[i] >= 0) {
+          pos[k] = have[i] + ((int)t - tok[i]);
+          const int col = pos[k] / a.page, first = (have[i] + a.page - 1) / a.page;
+          int p;
+          if (col >= first) {
+            p = listed((long long)taken + pg[i] + (col - first));
+          } else {  // a page the request already holds
+            p = a.bt[(long long)i * a.bt_stride + col];
+            if ((unsigned)p >= (unsigned)a.npages) p = -1;
+          }
+          if (p >= 0) slot[k] = p * a.page + (pos[k] - col * a.page);
+        }
+      }
+    }
+    if (vec && t0 + PT_TOKENS <= a.max_tokens) {
+      *(int4*)(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *(int4*)(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    } else {
+      for (int k = 0; k < PT_TOKENS && t0 + k < a.max_tokens; ++k) {
+        a.slots[t0 + k] = slot[k];
+        a.positions[t0 + k] = pos[k];
+      }
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t page_tables_launch(const PageTables& a, cudaStream_t stream) {
+  const size_t smem = ((size_t)3 * a.nseq + 2) * sizeof(int);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)((3 * kMaxTableRequests + 2) * sizeof(int)));
+    if (e != cudaSuccess) return e;
+  }
+  // as many CTAs as the tokens or requests fill, up to one cluster
+  const long long fill = ((long long)a.max_tokens / PT_TOKENS > a.nseq ? a.max_tokens / PT_TOKENS : a.nseq);
+  int ctas = 1;
+  while (ctas < PT_CLUSTER && (long long)ctas * PT_THREADS < fill) ctas <<= 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(PT_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ctas;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, page_tables_kernel, a);
+}
+
+}  // namespace w4b

@@ -26,6 +26,10 @@ enum : int {
   ST_FLASH_TIMEOUT = 301,         // flash decode: a pipeline wait ran out
   ST_PEER_TIMEOUT = 401,          // peer all-gather: a peer's slice never arrived
   ST_QUANT_INVALID = 501,         // device quantizer: a value or scale the host quantizer would have thrown on
+  ST_PAGES_EXHAUSTED = 601,       // page tables: the free list is too short; the missing entries are -1
+  ST_PAGES_INVALID = 602,         // page tables: a negative count, a request longer than its table row, too many tokens
+  ST_KV_WRITE_SLOT = 603,         // 8-bit cache write: a slot outside the pool, or a page's tokens out of order
+  ST_KV_PAGE = 604,               // 8-bit attention: a block-table entry outside the pool (its positions are left out)
 };
 
 // --------------------------------------------------------------------------

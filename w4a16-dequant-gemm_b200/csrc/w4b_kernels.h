@@ -41,6 +41,70 @@ cudaError_t quantize_mx_launch(const void* w, int f16, int N, int K, uint32_t* q
 cudaError_t quantize_f8_launch(const void* x, int f16, int rows, int D, int gs, long long out_mul, long long out_add,
                                uint8_t* q, __half* scales, int* status, cudaStream_t stream);
 
+// ---- page_tables.cu -----------------------------------------------------------
+constexpr int kMaxTableRequests = 16384;  // three ints of shared memory each
+struct PageTables {
+  const int* cached;
+  const int* fresh;
+  int nseq, page, npages;
+  const int* free_pages;
+  int nfree;
+  const int* taken_in;
+  int* taken_out;
+  int* bt;
+  int bt_stride;
+  int* seq_lens;
+  int* q_offsets;
+  int* slots;
+  int* positions;
+  int max_tokens;
+  int* status;
+};
+cudaError_t page_tables_launch(const PageTables& a, cudaStream_t stream);
+
+// ---- kv_write_b8.cu -----------------------------------------------------------
+struct KvWriteB8 {
+  const int* slots;
+  int T;
+  const void* k_new;  // FP16 or BF16, a row of H * D values every k_stride values
+  const void* v_new;
+  long long k_stride, v_stride;
+  int page, npages;
+  uint8_t* q_k;
+  float* s_k;
+  uint8_t* q_v;
+  float* s_v;
+  int window;  // tokens a CTA looks through for runs to write (set by the launcher)
+  int* status;
+};
+cudaError_t kv_write_b8_launch(const KvWriteB8& a, int H, int D, int bf16, int sm_count, cudaStream_t stream);
+
+// ---- attn_b8.cu ---------------------------------------------------------------
+struct AttnB8 {
+  const uint8_t* q_k;
+  const float* s_k;
+  const uint8_t* q_v;
+  const float* s_v;
+  int H, page, npages;  // key/value heads
+  const int* bt;
+  int bt_stride;
+  const int* seq_lens;
+  const int* q_offsets;  // null: one query token per sequence
+  int nseq, max_q, max_len;
+  const void* q;
+  long long q_stride;
+  int group;             // query heads per key/value head
+  float scale;
+  int causal;
+  void* out;
+  long long out_stride;
+  float* lse;            // may be null
+  void* ws;              // arrival counters (zero between launches), then partial results
+  int* status;
+};
+size_t attn_b8_ws_bytes(int sm_count);
+cudaError_t attn_b8_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaStream_t stream, int* launches);
+
 // ---- relayout.cu ---------------------------------------------------------------
 // The matrix zero-extended along K to Kp columns (Gp groups / blocks per row) in the same packed format.
 // fmt: 0 = W4 symmetric, 1 = W4 asymmetric, 2 = MXFP4 (gs ignored).
