@@ -334,7 +334,7 @@ int w4b_attn_single_w4(const w4b_kv_w4* p, const void* q, void* out, void* strea
  *   nothing gets zeros and -inf. Rows of out outside the sequences' tokens are left as they are.
  *   A block-table entry outside 0..npages-1 is read as a page without positions (status 604).
  *   Lengths above max_seq_len and tokens above max_q are cut off there.
- *   ws: w4b_attn_b8_workspace() bytes of device memory for this call (256-byte aligned, zero-filled
+ *   ws: w4b_attn_b8_workspace(max_q, Hq, H) bytes of device memory for this call (256-byte aligned, zero-filled
  *   once by the caller; every call leaves the zeros it needs). Calls that may overlap - on two
  *   streams, or two captured graphs - take different ones. NULL: library scratch, which is
  *   allocated by the first such call (before any capture), never replaced, and shared by all of
@@ -344,7 +344,7 @@ int w4b_page_tables(const int* cached, const int* fresh, int nseq, int page, int
                     int* q_offsets, int* slots, int* positions, int max_tokens, void* stream);
 int w4b_kv_write_b8(const w4b_kv_b8* p, const int* slots, int T, const void* k_new, const void* v_new,
                     long long k_stride, long long v_stride, int dtype, void* stream);
-long long w4b_attn_b8_workspace(void);
+long long w4b_attn_b8_workspace(int max_q, int Hq, int H);
 int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const int* seq_lens, const int* q_offsets,
                       int nseq, int max_q, int max_seq_len, const void* q, long long q_stride, int Hq, int dtype,
                       float scale, int causal, void* out, long long out_stride, float* lse, void* ws,

@@ -566,7 +566,7 @@ def test_attention_streams_and_graphs(nq):
     """Two captured graphs with a workspace each, replayed on two streams at once."""
     probs = [Problem([3000, 500], [nq, nq], 2, 4, 128, 16, F16, True, seed=20 + i) for i in range(2)]
     want = [p.run() for p in probs]
-    size = w4.attention_b8_workspace()
+    size = w4.attention_b8_workspace(nq, 8, 2)
     graphs, got, keep = [], [], []
     for p in probs:
         ws = torch.zeros(size, dtype=torch.uint8, device="cuda")

@@ -91,7 +91,7 @@ ABI = {
     "w4b_attn_single_w4": (_I, [C.POINTER(_KvW4), _P, _P, _P, _P, _P]),
     "w4b_page_tables": (_I, [_P, _P, _I, _I, _I, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _P]),
     "w4b_kv_write_b8": (_I, [C.POINTER(_KvB8), _P, _I, _P, _P, _L, _L, _I, _P]),
-    "w4b_attn_b8_workspace": (_L, []),
+    "w4b_attn_b8_workspace": (_L, [_I, _I, _I]),
     "w4b_attn_b8_paged": (_I, [C.POINTER(_KvB8), _P, _I, _P, _P, _I, _I, _I, _P, _L, _I, _I, C.c_float, _I, _P, _L, _P,
                                _P, _L, _P]),
     "w4b_peer_alloc": (_I, [C.c_size_t, C.POINTER(_P), _P]),
@@ -344,11 +344,11 @@ def kv_write_b8(p: DeviceKVB8, slots, T, k_new, v_new, k_stride, v_stride, dtype
     _check(lib.w4b_kv_write_b8(C.byref(p._c()), slots, T, k_new, v_new, k_stride, v_stride, dtype, stream))
 
 
-def attention_b8_workspace() -> int:
-    """Bytes of a workspace of attention_b8_paged on the current device."""
-    n = lib.w4b_attn_b8_workspace()
+def attention_b8_workspace(max_q, Hq, H) -> int:
+    """Bytes of a workspace for attention_b8_paged calls of up to max_q query tokens a sequence, on this device."""
+    n = lib.w4b_attn_b8_workspace(max_q, Hq, H)
     if n < 0:
-        raise CudaError(lib.w4b_last_error().decode())
+        raise InvalidArgument(lib.w4b_last_error().decode())
     return n
 
 

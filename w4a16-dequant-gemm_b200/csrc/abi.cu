@@ -81,7 +81,7 @@ struct DeviceCtx {
   Scratch attn_ws;        // (m, l, acc[D]) partials of split sequences
   Scratch io_x, io_c;     // device staging of the host-buffer entry
   Scratch gemm_xpad;      // zero-padded activation rows of the padded-K entries
-  Scratch b8_ws;          // counters and partial results of the 8-bit paged attention: one size, never replaced
+  Scratch b8_ws, b8_chunk_ws;  // counters and partial results of the 8-bit paged attention: one size, never replaced
 };
 
 constexpr int kMaxDevices = 64;
@@ -772,10 +772,20 @@ int w4b_kv_write_b8(const w4b_kv_b8* p, const int* slots, int T, const void* k_n
   return W4B_OK;
 }
 
-long long w4b_attn_b8_workspace(void) {
+namespace {
+// The two kernels' regions of a workspace; the second only for calls whose largest sequence reaches the chunk kernel.
+size_t b8_ws_part(int sm_count) { return (attn_b8_ws_bytes(sm_count) + 255) / 256 * 256; }
+bool b8_chunked(long long max_q, int group) { return max_q * group >= kChunkRows; }
+}  // namespace
+
+long long w4b_attn_b8_workspace(int max_q, int Hq, int H) {
+  if (max_q < 1 || H < 1 || Hq < 1 || Hq % H != 0) {
+    fail(W4B_INVALID, "attention b8 workspace: bad query shape");
+    return -1;
+  }
   DeviceCtx* ctx = nullptr;
   if (get_ctx(&ctx)) return -1;
-  return (long long)attn_b8_ws_bytes(ctx->sm_count);
+  return (long long)(b8_ws_part(ctx->sm_count) + (b8_chunked(max_q, Hq / H) ? attn_b8_chunk_ws_bytes(ctx->sm_count) : 0));
 }
 
 int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const int* seq_lens, const int* q_offsets, int nseq,
@@ -798,12 +808,17 @@ int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const in
   if (ws && ((uintptr_t)ws & 255u)) INVALID("%s: the workspace must be 256-byte aligned", who);
   DeviceCtx* ctx = nullptr;
   if (int rc = get_ctx(&ctx)) return rc;
-  const size_t need = attn_b8_ws_bytes(ctx->sm_count);
+  const bool chunked = b8_chunked(max_q, Hq / p->H);
+  const size_t first = b8_ws_part(ctx->sm_count), second = chunked ? attn_b8_chunk_ws_bytes(ctx->sm_count) : 0;
+  void* chunk_ws = nullptr;
   if (ws) {
-    if (ws_bytes < (long long)need) INVALID("%s: workspace of %lld bytes, %zu are needed", who, ws_bytes, need);
+    if (ws_bytes < (long long)(first + second)) INVALID("%s: workspace of %lld bytes, %zu are needed", who, ws_bytes, first + second);
+    chunk_ws = (uint8_t*)ws + first;
   } else {
-    CUDA_TRY(ctx->b8_ws.reserve(need, true), "attention workspace");
+    CUDA_TRY(ctx->b8_ws.reserve(first, true), "attention workspace");
+    CUDA_TRY(ctx->b8_chunk_ws.reserve(second, true), "attention workspace");
     ws = ctx->b8_ws.ptr;
+    chunk_ws = ctx->b8_chunk_ws.ptr;
   }
   AttnB8 a;
   memset(&a, 0, sizeof(a));
@@ -830,6 +845,9 @@ int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const in
   a.out_stride = out_stride;
   a.lse = lse;
   a.ws = ws;
+  a.chunk_ws = chunk_ws;
+  a.chunk_rows = kChunkRows;
+  a.page_div = FastDiv::of(p->page);
   a.status = ctx->status;
   int launches = 0;
   CUDA_TRY(attn_b8_launch(a, p->D, dtype == W4B_DTYPE_BF16, ctx->sm_count, (cudaStream_t)stream, &launches), who);

@@ -24,11 +24,7 @@
 // Split: all work - 64-position units of all (sequence, head, column tile) rows in order - is cut into equal ranges,
 // one per CTA, whatever the lengths; the lengths are on the device, so every CTA sums them itself. A row that spans
 // CTAs is joined by whichever of them arrives last, in CTA order (bit-identical from run to run).
-#include <cuda_bf16.h>
-#include <float.h>
-
-#include "w4b_common.cuh"
-#include "w4b_kernels.h"
+#include "attn_b8.cuh"
 
 namespace w4b {
 namespace {
@@ -39,12 +35,6 @@ constexpr int AB_CTAS_PER_SM = 4;
 constexpr int AB_STAGES = 3;
 constexpr int AB_UNIT = 64;      // positions per work unit: one block of 16 per warp
 constexpr int AB_MAX_COLS = 16;  // query rows per column tile
-constexpr int AB_MAX_D = 128;
-constexpr float AB_LOG2E = 1.4426950408889634f;
-constexpr float AB_LN2 = 0.6931471805599453f;
-constexpr float AB_SLACK = 8.0f;   // how far a weight's exponent may exceed the reference point
-constexpr float AB_NONE = -1e30f;  // reference point of a column that has seen nothing
-
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -71,43 +61,10 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// bytes 0, 1 (lo) and 2, 3 (hi) of w to half2 each
-__device__ __forceinline__ void e4m3x4_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n"
-      ".reg .b16 a, b;\n"
-      "mov.b32 {a, b}, %2;\n"
-      "cvt.rn.f16x2.e4m3x2 %0, a;\n"
-      "cvt.rn.f16x2.e4m3x2 %1, b;\n"
-      "}\n"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// What a sequence asks for, with the device-side values held inside what the launch was sized for.
-struct SeqInfo {
-  int len, q0, nq;
-};
-__device__ __forceinline__ SeqInfo seq_info(const AttnB8& a, int i) {
-  SeqInfo s;
-  s.len = min(max(a.seq_lens[i], 0), a.max_len);
-  s.q0 = a.q_offsets ? a.q_offsets[i] : i;
-  s.nq = a.q_offsets ? min(max(a.q_offsets[i + 1] - s.q0, 0), a.max_q) : 1;
-  return s;
-}
-
 template <int NC>
 __device__ __forceinline__ long long seq_units(const AttnB8& a, const SeqInfo& s, int& tiles, int& units) {
-  tiles = (s.nq * a.group + NC - 1) / NC;
+  const int rows = s.nq * a.group;
+  tiles = rows < a.chunk_rows ? (rows + NC - 1) / NC : 0;  // the others are the chunk kernel's
   units = max(1, (s.len + AB_UNIT - 1) / AB_UNIT);
   return (long long)a.H * tiles * units;
 }
@@ -193,7 +150,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
   long long u = u_begin;
 
   int* counters = (int*)a.ws;
-  float* parts = (float*)((uint8_t*)a.ws + 4 * (((size_t)gridDim.x + 63) / 64 * 64));
+  float* parts = (float*)((uint8_t*)a.ws + counter_bytes((int)gridDim.x));
   const uint32_t ring = smem_u32(smem) + wid * C::RING;
 
   while (u < u_end) {
@@ -237,8 +194,6 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
           qf[t][i][1] = v.y;
         }
       } else {
-        // BF16 to FP16 by a power of two of the row's own: its largest value lands in [2^14, 2^15), what falls
-        // below the half range is 2^-39 of it
         uint2 v[C::KSTEPS];
         uint32_t top = 0;
 #pragma unroll
@@ -249,17 +204,13 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
         top = max(top & 0xFFFFu, top >> 16);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = (int)(top >> 7);  // biased exponent
-        const int k = min(max(141 - e, -100), 100);  // 127 + 14 - e
-        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
-        scale_row = __uint_as_float((uint32_t)(127 - k) << 23);
+        float up;
+        bf16_row_scale(top, up, scale_row);
 #pragma unroll
         for (int i = 0; i < C::KSTEPS; ++i) {
           const uint32_t w[2] = {v[i].x, v[i].y};
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            qf[t][i][j] = h2_as_u32(__floats2half2_rn(__uint_as_float(w[j] << 16) * up,
-                                                      __uint_as_float(w[j] & 0xFFFF0000u) * up));
+          for (int j = 0; j < 2; ++j) qf[t][i][j] = bf16x2_to_h2(w[j], up);
         }
       }
 #pragma unroll
@@ -291,13 +242,13 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     const int* bt = a.bt + (long long)seq * a.bt_stride;
     const size_t slab = (size_t)head * a.npages;
     auto position = [&](int j) { return p_begin + (wid + j * AB_WARPS) * 16; };
-    auto page_of = [&](int j) { return j < mine_n ? bt[position(j) / a.page] : 0; };
+    auto page_of = [&](int j) { return j < mine_n ? bt[a.page_div.div(position(j))] : 0; };
     auto issue = [&](int j, int pg) {
       const uint32_t st = ring + (j % AB_STAGES) * C::STAGE;
       if (j < mine_n) {
         const int p0 = position(j);
         const bool good = (unsigned)pg < (unsigned)a.npages;
-        const size_t r = (slab + (good ? pg : 0)) * a.page + (p0 - p0 / a.page * a.page);
+        const size_t r = (slab + (good ? pg : 0)) * a.page + (p0 - a.page_div.div(p0) * a.page);
         const uint8_t* ks = a.q_k + r * D;
         const uint8_t* vs = a.q_v + r * D;
 #pragma unroll
@@ -454,22 +405,14 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     auto store_row = [&](int n, int d, const float v[8], float ms, float ls) {
       // d: first of eight dims; v unnormalised
       const int r = tile * NC + n, tq = r / a.group, hq = head * a.group + (r - tq * a.group);
-      const float inv = ls > 0.0f ? 1.0f / ls : (ls == 0.0f ? 0.0f : ls);  // nothing seen: zeros; NaN stays
+      const float inv = row_norm(ls);
       uint32_t h[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = v[2 * i] * inv, q = v[2 * i + 1] * inv;
-        if (BF16) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(p, q);
-          h[i] = *(const uint32_t*)&b;
-        } else {
-          h[i] = h2_as_u32(__floats2half2_rn(p, q));
-        }
-      }
+      for (int i = 0; i < 4; ++i) h[i] = pack_out<BF16>(v[2 * i] * inv, v[2 * i + 1] * inv);
       *(uint4*)((uint16_t*)a.out + (long long)(s.q0 + tq) * a.out_stride + (size_t)hq * D + d) =
           make_uint4(h[0], h[1], h[2], h[3]);
       if (a.lse && d == 0)
-        a.lse[(long long)(s.q0 + tq) * (a.H * a.group) + hq] = ls == 0.0f ? -INFINITY : (ms + log2f(ls)) * AB_LN2;
+        a.lse[(long long)(s.q0 + tq) * (a.H * a.group) + hq] = row_lse(ms, ls);
     };
     float* part = parts + (size_t)(2 * cta + (r0 == 0 ? 1 : 0)) * C::PART;
     for (int e = tid; e < NC * LANES; e += AB_THREADS) {
@@ -552,7 +495,6 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
 }
 
 int attn_b8_grid(int sm_count) { return AB_CTAS_PER_SM * sm_count; }
-size_t counter_bytes(int grid) { return 4 * (((size_t)grid + 63) / 64 * 64); }
 
 template <int D, int NT, bool BF16>
 cudaError_t launch(const AttnB8& a, int sm_count, cudaStream_t stream) {
@@ -572,8 +514,15 @@ size_t attn_b8_ws_bytes(int sm_count) {
 }
 
 cudaError_t attn_b8_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaStream_t stream, int* launches) {
-  const bool wide = (long long)a.max_q * a.group > 8;
+  const long long rows = (long long)a.max_q * a.group;
+  const bool wide = rows > 8;
   *launches = 1;
+  if (rows >= a.chunk_rows) {
+    const cudaError_t e = attn_b8_chunk_launch(a, D, bf16, sm_count, stream);
+    // one sequence, or no row count below the threshold: nothing is left for the kernel below
+    if (e != cudaSuccess || a.nseq == 1) return e;
+    *launches = 2;
+  }
 #define W4B_GO(DD)                                                                                      \
   (bf16 ? (wide ? launch<DD, 2, true>(a, sm_count, stream) : launch<DD, 1, true>(a, sm_count, stream)) \
         : (wide ? launch<DD, 2, false>(a, sm_count, stream) : launch<DD, 1, false>(a, sm_count, stream)))

@@ -1,0 +1,75 @@
+// What the two kernels of attention over a paged 8-bit cache share (attn_b8.cu, attn_b8_chunk.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "w4b_common.cuh"
+#include "w4b_kernels.h"
+
+namespace w4b {
+
+constexpr int AB_MAX_D = 128;
+constexpr float AB_LOG2E = 1.4426950408889634f;
+constexpr float AB_LN2 = 0.6931471805599453f;
+constexpr float AB_SLACK = 8.0f;   // how far a weight's exponent may exceed the reference point
+constexpr float AB_NONE = -1e30f;  // reference point of a row that has seen nothing
+
+__host__ __device__ __forceinline__ size_t counter_bytes(int grid) { return 4 * (((size_t)grid + 63) / 64 * 64); }
+
+// bytes 0, 1 (lo) and 2, 3 (hi) of w to half2 each
+__device__ __forceinline__ void e4m3x4_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n"
+      ".reg .b16 a, b;\n"
+      "mov.b32 {a, b}, %2;\n"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n"
+      "}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// BF16 query rows become FP16 by a power of two of the row's own: with `top` the largest |q| (bits) its largest value
+// lands in [2^14, 2^15), and what falls below the half range is 2^-39 of it. scale_row undoes it in the scores.
+__device__ __forceinline__ void bf16_row_scale(uint32_t top, float& up, float& scale_row) {
+  const int k = min(max(141 - (int)(top >> 7), -100), 100);  // 127 + 14 - the biased exponent
+  up = __uint_as_float((uint32_t)(127 + k) << 23);
+  scale_row = __uint_as_float((uint32_t)(127 - k) << 23);
+}
+__device__ __forceinline__ uint32_t bf16x2_to_h2(uint32_t w, float up) {
+  return h2_as_u32(__floats2half2_rn(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xFFFF0000u) * up));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_out(float x, float y) {
+  if (BF16) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t*)&b;
+  }
+  return h2_as_u32(__floats2half2_rn(x, y));
+}
+// 1 / l; a row that saw nothing gives zeros, NaN stays
+__device__ __forceinline__ float row_norm(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * AB_LN2; }
+
+// What a sequence asks for, with the device-side values held inside what the launch was sized for.
+struct SeqInfo {
+  int len, q0, nq;
+};
+__device__ __forceinline__ SeqInfo seq_info(const AttnB8& a, int i) {
+  SeqInfo s;
+  s.len = min(max(a.seq_lens[i], 0), a.max_len);
+  s.q0 = a.q_offsets ? a.q_offsets[i] : i;
+  s.nq = a.q_offsets ? min(max(a.q_offsets[i + 1] - s.q0, 0), a.max_q) : 1;
+  return s;
+}
+
+}  // namespace w4b

@@ -79,13 +79,29 @@ struct KvWriteB8 {
 };
 cudaError_t kv_write_b8_launch(const KvWriteB8& a, int H, int D, int bf16, int sm_count, cudaStream_t stream);
 
-// ---- attn_b8.cu ---------------------------------------------------------------
+// ---- attn_b8.cu, attn_b8_chunk.cu ---------------------------------------------
+// n / d for 0 <= n < 2^31 by a multiplication: with m = floor(2^(31 + s) / d) + 1, s = ceil(log2 d), the error
+// n * (m * d - 2^(31 + s)) / (d * 2^(31 + s)) stays below 1 / d.
+struct FastDiv {
+  unsigned m;
+  int s;
+  static FastDiv of(int d) {
+    FastDiv f;
+    for (f.s = 0; (1LL << f.s) < d; ++f.s) {}
+    f.m = (unsigned)((1ULL << (31 + f.s)) / (unsigned)d + 1);
+    return f;
+  }
+  __host__ __device__ __forceinline__ int div(int n) const {
+    return (int)(((unsigned long long)(unsigned)n * m) >> (31 + s));
+  }
+};
 struct AttnB8 {
   const uint8_t* q_k;
   const float* s_k;
   const uint8_t* q_v;
   const float* s_v;
   int H, page, npages;  // key/value heads
+  FastDiv page_div;
   const int* bt;
   int bt_stride;
   const int* seq_lens;
@@ -100,9 +116,14 @@ struct AttnB8 {
   long long out_stride;
   float* lse;            // may be null
   void* ws;              // arrival counters (zero between launches), then partial results
+  void* chunk_ws;        // the same for the chunk kernel
+  int chunk_rows;        // sequences with at least this many query rows per key/value head are the chunk kernel's
   int* status;
 };
+constexpr int kChunkRows = 48;
 size_t attn_b8_ws_bytes(int sm_count);
+size_t attn_b8_chunk_ws_bytes(int sm_count);
+cudaError_t attn_b8_chunk_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaStream_t stream);
 cudaError_t attn_b8_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaStream_t stream, int* launches);
 
 // ---- relayout.cu ---------------------------------------------------------------
