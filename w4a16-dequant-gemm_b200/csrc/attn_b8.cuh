@@ -11,7 +11,7 @@ namespace w4b {
 constexpr int AB_MAX_D = 128;
 constexpr float AB_LOG2E = 1.4426950408889634f;
 constexpr float AB_LN2 = 0.6931471805599453f;
-constexpr float AB_SLACK = 8.0f;   // how far a weight's exponent may exceed the reference point
+constexpr float AB_SLACK = 14.0f;  // how far the exponent of a weight may exceed the reference point (halves end at 2^16)
 constexpr float AB_NONE = -1e30f;  // reference point of a row that has seen nothing
 
 __host__ __device__ __forceinline__ size_t counter_bytes(int grid) { return 4 * (((size_t)grid + 63) / 64 * 64); }

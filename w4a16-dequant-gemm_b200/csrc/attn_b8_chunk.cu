@@ -1,24 +1,28 @@
 // Attention over a paged 8-bit cache for sequences with many query rows per key/value head (prompt chunks, encoder
 // states): the same operator as attn_b8.cu, bound by the tensor pipe instead of HBM, on tcgen05.
 //
-// One CTA works on 128 query rows (token-major: row = token * group + head of the group) of one sequence and
-// key/value head, and walks the positions in tiles of 64:
-//   S = Q K^T        tcgen05.mma M = 128, N = 64; A = Q from tensor memory, B = the K tile in shared memory
+// One CTA per SM works on a group of up to 256 query rows (token-major: row = token * group + head of the group) of one
+// sequence and key/value head, and walks the positions in tiles of 64. Two warpgroups hold 128 rows each:
+//   S = Q K^T        tcgen05.mma M = 128, N = 64; B = the K tile in shared memory
 //   w = 2^(S * s_k * scale * log2 e + log2 s_v - m)      (why V's scale goes into the weights: attn_b8.cu)
-//   O += w V         M = 128, N = D, K = 64; A = w from tensor memory (over S), B = the V tile
-// Both A operands come from tensor memory because that form issues a 128 x 128 x 16 product every 74 cycles against
-// 103 with A in shared memory (64 ideal; measured alone), and because it leaves shared memory to the conversion.
-//   warps 0-3  one thread per query row (its TMEM lane): no reduction across threads anywhere. The reference point m
-//              moves only when a score exceeds it by 2^8 (see attn_b8.cu); then O is rescaled in place.
-//   warps 4-7  E4M3 -> FP16 (exact): 16-byte loads of the next tile in flight while the current one is written to
-//              swizzled operand tiles. K is K-major; V is stored the same way (row = position) and read MN-major.
-//   One elected thread of warp 0 issues the MMAs, when the four warps' weights are in place: it has nothing else to do
-//   until the next scores are there, and with eight warps a thread may use 128 registers. (elect.sync, not "lane == 0":
-//   with a plain thread test an instruction took 92 cycles to issue whatever its size.)
-// Two CTAs per SM (TMEM: S 64 + O 128 + Q 64 = 256 columns each): one's softmax overlaps the other's products.
+//   O += w V         M = 128, N = D, K = 64; A = w from tensor memory, B = the V tile
+// A group of at most 128 rows is given to both warpgroups, which take the tiles in turn and join their results in
+// shared memory.
+//   warps 0-7   one thread per query row (its TMEM lane): no reduction across threads anywhere. The reference point m
+//               moves only when a score exceeds it by 2^14 (see attn_b8.cu); then O is rescaled in place.
+//   warps 8-11  E4M3 -> FP16 (exact), once for both warpgroups: 16-byte loads two tiles ahead in registers, written to
+//               swizzled operand tiles. K is K-major; V is stored the same way (row = position) and read MN-major.
+//   warp 12     one elected thread issues all MMAs: the scores of a warpgroup's next tile as soon as it has read the
+//               present ones, so that they run under its exponentials, then the weights' product. (A warpgroup that
+//               issues for itself waits out its own products: 2900 cycles a tile instead of XXXX. elect.sync, not
+//               "lane == 0": with a plain thread test an instruction took 92 cycles to issue whatever its size.)
+// Tensor memory: S 2 x 64, w 2 x 32, O 2 x 128 columns and the first 64 dims of Q, 2 x 32; with D = 128 the other half
+// of Q is in shared memory. An A operand in tensor memory is worth having: 42 cycles for 128 x 64 x 16 against 72 with
+// A in shared memory (32 ideal; measured alone).
+// Registers: 512 threads of 128 at launch, split 160 / 160 / 112 / 80 between the warpgroups.
 //
-// Split: units of one tile over all (sequence, head, row tile) in order, cut into equal ranges, as in attn_b8.cu; the
-// causal limit of every row tile is in the count.
+// Split: units of one tile (two, for a group that both warpgroups share) over all (sequence, head, row group) in
+// order, cut into equal ranges, as in attn_b8.cu; the causal limit of every group is in the count.
 #include <cuda_bf16.h>
 #include <float.h>
 
@@ -27,12 +31,12 @@
 namespace w4b {
 namespace {
 
-constexpr int AC_ROWS = 128;
-constexpr int AC_TILE = 64;   // positions per tile
-constexpr int AC_THREADS = 256;
+constexpr int AC_ROWS = 128;          // query rows per warpgroup
+constexpr int AC_GROUP = 2 * AC_ROWS;  // per CTA
+constexpr int AC_TILE = 64;            // positions per tile
+constexpr int AC_THREADS = 512;
 constexpr int AC_WARPS = AC_THREADS / 32;
-constexpr int AC_CTAS_PER_SM = 2;
-constexpr int AC_MIN_UNITS = 4;  // tiles per CTA below which no further split pays
+constexpr int AC_MIN_UNITS = 4;        // units per CTA below which no further split pays
 
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -59,6 +63,16 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
       "}\n" ::"r"(tmem_d),
       "r"(tmem_a), "l"(db), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
@@ -90,32 +104,58 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Positions the rows of a row tile see, and its tiles.
-struct RowTile {
-  int rows;      // query rows in use
-  int end;       // positions any row sees
-  int all_see;   // positions every row sees
-  int units;     // tiles (at least one: a row tile that sees nothing still writes its zeros)
+// two FP32 values in one register pair: one instruction for both
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 pair(float a) { return pair(a, a); }
+__device__ __forceinline__ float lo(f32x2 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi(f32x2 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A group of query rows, the positions it sees, and its units.
+struct RowGroup {
+  int rows;    // query rows in use
+  int tiles;   // position tiles any row sees
+  int units;   // at least one: a group that sees nothing still writes its zeros
+  bool split;  // both warpgroups share the rows
 };
-__device__ __forceinline__ RowTile row_tile(const AttnB8& a, const SeqInfo& s, int qt) {
-  RowTile t;
-  const int first = qt * AC_ROWS;
-  t.rows = min(AC_ROWS, s.nq * a.group - first);
-  const int before = s.len - s.nq;
-  t.end = a.causal ? min(s.len, max(0, before + (first + t.rows - 1) / a.group + 1)) : s.len;
-  t.all_see = a.causal ? max(0, before + first / a.group + 1) : s.len;
-  t.units = max(1, (t.end + AC_TILE - 1) / AC_TILE);
+__device__ __forceinline__ RowGroup row_group(const AttnB8& a, const SeqInfo& s, int gi) {
+  RowGroup t;
+  const int first = gi * AC_GROUP;
+  t.rows = min(AC_GROUP, s.nq * a.group - first);
+  t.split = t.rows <= AC_ROWS;
+  const int end = a.causal ? min(s.len, max(0, s.len - s.nq + (first + t.rows - 1) / a.group + 1)) : s.len;
+  t.tiles = max(1, (end + AC_TILE - 1) / AC_TILE);
+  t.units = t.split ? (t.tiles + 1) / 2 : t.tiles;
   return t;
 }
-__device__ __forceinline__ int row_tiles(const AttnB8& a, const SeqInfo& s) {
+__device__ __forceinline__ int row_groups(const AttnB8& a, const SeqInfo& s) {
   const int rows = s.nq * a.group;
-  return rows >= a.chunk_rows ? (rows + AC_ROWS - 1) / AC_ROWS : 0;
+  return rows >= a.chunk_rows ? (rows + AC_GROUP - 1) / AC_GROUP : 0;
 }
 // Units of one head of a sequence, by a warp (the same value in every lane).
 __device__ __forceinline__ long long head_units(const AttnB8& a, const SeqInfo& s, int lane) {
-  const int n = row_tiles(a, s);
+  const int n = row_groups(a, s);
   long long sum = 0;
-  for (int qt = lane; qt < n; qt += 32) sum += row_tile(a, s, qt).units;
+  for (int gi = lane; gi < n; gi += 32) sum += row_group(a, s, gi).units;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   return sum;
@@ -124,27 +164,63 @@ __device__ __forceinline__ long long head_units(const AttnB8& a, const SeqInfo& 
 template <int D>
 struct ChunkSmem {
   static constexpr int TILE_BYTES = AC_TILE * D * 2;  // an FP16 operand tile: D / 64 blocks of 64 rows x 128 bytes
-  static constexpr int STAGES = 2;
-  static constexpr int META = 4 * 4 * 16;              // four tiles of four blocks of 16 positions
-  static constexpr int K_OFF = 0, V_OFF = STAGES * TILE_BYTES, META_OFF = 2 * STAGES * TILE_BYTES;
-  static constexpr int BAR_OFF = META_OFF + META;
-  static constexpr int BYTES = BAR_OFF + 128 + 1024;   // + alignment
+  static constexpr int STAGES = 4;
+  static constexpr int METAS = 2 * STAGES;             // a tile's factors outlive its stage: they are read after the scores
+  static constexpr int META = METAS * 4 * 16;          // per tile: four blocks of 16 positions
+  static constexpr int JOIN = AC_ROWS * (D + 2) * 4;   // the second warpgroup's result of a shared group
+  // dims 64 .. 127 of both warpgroups' query rows (D = 128) share their place with the join buffer
+  static constexpr int K_OFF = 0, V_OFF = STAGES * TILE_BYTES, Q_OFF = 2 * STAGES * TILE_BYTES, JOIN_OFF = Q_OFF;
+  static constexpr int META_OFF = JOIN_OFF + JOIN, BAR_OFF = META_OFF + META;
+  static constexpr int BYTES = BAR_OFF + 256 + 1024;   // + alignment
 };
 
 // where a CTA's range of units starts
 struct RangeStart {
   long long u_begin, u_end, total, ctas;
-  int seq, head, qt, r0;
+  int seq, head, gi, r0;
+};
+
+// A role's walk over its CTA's row groups.
+struct Walk {
+  int left;  // units still to do
+  int seq, head, gi, r0;
+  int it;    // tiles so far: stage and phase of the rings
+  SeqInfo s;
+  RowGroup t;
+  int n_units, tile0, n_tiles;  // of the present group
+  __device__ __forceinline__ explicit Walk(const AttnB8& a, const RangeStart& b)
+      : left((int)(b.u_end - b.u_begin)), seq(b.seq), head(b.head), gi(b.gi), r0(b.r0), it(0), s(seq_info(a, b.seq)) {}
+  __device__ __forceinline__ bool more(const AttnB8& a) {
+    if (left <= 0) return false;
+    while (row_groups(a, s) == 0) s = seq_info(a, ++seq);  // sequences of the other kernel
+    t = row_group(a, s, gi);
+    n_units = min(t.units - r0, left);
+    tile0 = t.split ? 2 * r0 : r0;
+    n_tiles = t.split ? min(2 * n_units, t.tiles - tile0) : n_units;
+    return true;
+  }
+  __device__ __forceinline__ void next(const AttnB8& a) {
+    left -= n_units;
+    it += n_tiles;
+    r0 = 0;
+    if (++gi == row_groups(a, s)) {
+      gi = 0;
+      if (++head == a.H) {
+        head = 0;
+        if (left > 0) s = seq_info(a, ++seq);
+      }
+    }
+  }
 };
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kernel(const AttnB8 a) {
+__global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const AttnB8 a) {
   using L = ChunkSmem<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long wsum[AC_WARPS];
   __shared__ RangeStart start;
   __shared__ uint32_t tmem_slot;
-  __shared__ int is_last;
+  __shared__ int is_last[2];
   const int tid = threadIdx.x, lane = tid & 31, wid = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t sm = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smp = smem_raw + (sm - smem_u32(smem_raw));
@@ -179,10 +255,10 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
       }
       const int head = (int)(off / hu);
       off -= (long long)head * hu;
-      int qt = 0;
-      for (;; qt += 32) {  // 32 row tiles at a time
-        const int n = row_tiles(a, s);
-        long long v = qt + lane < n ? row_tile(a, s, qt + lane).units : 0, x = v;
+      int gi = 0;
+      for (;; gi += 32) {  // 32 groups at a time
+        const int n = row_groups(a, s);
+        long long v = gi + lane < n ? row_group(a, s, gi + lane).units : 0, x = v;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const long long o = __shfl_up_sync(0xffffffffu, x, d);
@@ -192,34 +268,43 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
         if (in != 0) {
           const int k = __ffs(in) - 1;
           off -= __shfl_sync(0xffffffffu, x - v, k);
-          qt += k;
+          gi += k;
           break;
         }
         off -= __shfl_sync(0xffffffffu, x, 31);
       }
-      if (lane == 0) start = RangeStart{ub, ue, T, G, i, head, qt, (int)off};
+      if (lane == 0) start = RangeStart{ub, ue, T, G, i, head, gi, (int)off};
     }
   }
 
   // ---- barriers, tensor memory ---------------------------------------------------------------------------------
   const uint32_t bars = sm + L::BAR_OFF;
   auto k_full = [&](int s) { return bars + 8u * s; };
-  auto k_free = [&](int s) { return bars + 16u + 8u * s; };
-  auto v_full = [&](int s) { return bars + 32u + 8u * s; };
-  auto v_free = [&](int s) { return bars + 48u + 8u * s; };
-  const uint32_t s_full = bars + 64u, o_done = bars + 72u;
+  auto k_free = [&](int s) { return bars + 32u + 8u * s; };
+  auto v_full = [&](int s) { return bars + 64u + 8u * s; };
+  auto v_free = [&](int s) { return bars + 96u + 8u * s; };
+  auto s_full = [&](int w) { return bars + 128u + 8u * w; };   // scores are there
+  auto s_free = [&](int w) { return bars + 144u + 8u * w; };   // scores have been read
+  auto w_full = [&](int w) { return bars + 160u + 8u * w; };   // weights are there
+  auto o_done = [&](int w) { return bars + 176u + 8u * w; };   // their product is done: O may be read, w overwritten
+  auto q_full = [&](int w) { return bars + 192u + 8u * w; };   // query rows are there
   if (tid == 0) {
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(k_full(s), 4);
+    for (int s = 0; s < L::STAGES; ++s) {
+      mbar_init(k_full(s), 4);  // the conversion warps
       mbar_init(k_free(s), 1);
       mbar_init(v_full(s), 4);
       mbar_init(v_free(s), 1);
     }
-    mbar_init(s_full, 2);   // the MMAs' completion and the issuing thread itself (for the tile's factors)
-    mbar_init(o_done, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full(w), 2);  // the MMAs' completion and the issuing thread itself (for the tile's factors)
+      mbar_init(s_free(w), 4);
+      mbar_init(w_full(w), 4);
+      mbar_init(o_done(w), 1);
+      mbar_init(q_full(w), 4);
+    }
     mbar_init_fence();
   }
-  constexpr uint32_t COLS = 256;
+  constexpr uint32_t COLS = 512;
   if (wid == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(COLS)
                  : "memory");
@@ -229,141 +314,201 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
   __syncthreads();
   tc_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  const uint32_t t_s = tmem, t_q = tmem + 64, t_o = tmem + 128;  // S (and the weights over it), Q, O
 
-  long long u = start.u_begin;
-  const long long u_end = start.u_end, T = start.total, G = start.ctas;
-  int seq = start.seq, head = start.head, qt = start.qt, r0 = start.r0;
-  SeqInfo s = seq_info(a, seq);
-  int it = 0;        // tiles so far: stage and phase of every ring
-  // A wait that gave up: from there on this thread only walks through, so that every barrier of the four softmax
-  // warps is met by all of them.
+  // A wait that gave up: from there on this thread only walks through, so that every barrier of the warpgroups is met
+  // by all of them.
   bool ok = true;
-
-  while (u < u_end) {
-    while (row_tiles(a, s) == 0) s = seq_info(a, ++seq);  // sequences of the other kernel
-    const RowTile t = row_tile(a, s, qt);
-    const int r1 = (int)min((long long)t.units, r0 + (u_end - u));
-    const int n_tiles = r1 - r0;
-
-    if (wid >= 4) {
-      // ------------------------------ conversion ------------------------------
-      constexpr int PIECES = D / 16, PASSES = AC_TILE * PIECES / 128;
-      const int ct = tid - 128;
-      const int* bt = a.bt + (long long)seq * a.bt_stride;
-      const size_t slab = (size_t)head * a.npages;
-      uint4 kr[PASSES], vr[PASSES];
-      float sk = 0.0f, sv = -1.0f;  // of block ct of the tile (threads 0-3)
-      auto load = [&](int r) {
-        const int p0 = r * AC_TILE;
+  // Registers: 128 threads x (160 + 160 + 112 + 80) = the 512 x 128 of the launch.
+  if (wid >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    // ------------------------------ MMA issue ------------------------------
+    if (wid == 12 && elect_one()) {
+      int mine = 0, other = 0, segments = 0;  // tiles of the warpgroups, row groups so far: phases
+      for (Walk k(a, start); k.more(a); k.next(a)) {
+        const RowGroup& t = k.t;
+        const int n_tiles = k.n_tiles, it = k.it;
+        // D = F32, A = B = F16; S: B (K) K-major; O: B (V) MN-major
+        constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(AC_TILE >> 3) << 17) | ((uint32_t)(AC_ROWS >> 4) << 24);
+        constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(AC_ROWS >> 4) << 24);
+        const int n[2] = {t.split ? (n_tiles + 1) / 2 : n_tiles, t.split ? n_tiles / 2 : n_tiles};
+        auto wait = [&](uint32_t bar, int phase) {
+          ok = ok && mbar_wait(bar, (uint32_t)phase & 1u, a.status, ST_FLASH_TIMEOUT);
+        };
+        auto scores = [&](int w, int i) {  // of the warpgroup's tile i
+          const int j = it + (t.split ? 2 * i + w : i), st = j % L::STAGES, c = (w ? other : mine) + i;
+          if (t.split || w == 0) wait(k_full(st), j / L::STAGES);
+          if (c > 0) wait(s_free(w), c - 1);
+          if (!ok) return;
+          tc_after_sync();
+          const uint32_t t_s = tmem + 64 * w, t_q = tmem + 192 + 32 * w;
+          const uint64_t db = operand_desc(sm + L::K_OFF + st * L::TILE_BYTES, 1);
+          const uint64_t da = operand_desc(sm + L::Q_OFF + w * (AC_ROWS * 128), 1);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t b = db + (uint64_t)((k >> 2) * (AC_TILE * 128 / 16) + (k & 3) * 2);
+            if (k < 4) mma_ts(t_s, t_q + 8 * k, b, id_s, k > 0);
+            else mma_ss(t_s, da + (uint64_t)((k & 3) * 2), b, id_s, true);
+          }
+          if (t.split || w == 1) mma_commit(k_free(st));
+          mma_commit(s_full(w));
+          mbar_arrive(s_full(w));
+        };
+        auto values = [&](int w, int i) {
+          const int j = it + (t.split ? 2 * i + w : i), st = j % L::STAGES, c = (w ? other : mine) + i;
+          if (t.split || w == 0) wait(v_full(st), j / L::STAGES);
+          wait(w_full(w), c);
+          if (!ok) return;
+          tc_after_sync();
+          const uint32_t t_w = tmem + 128 + 32 * w, t_o = tmem + 256 + 128 * w;
+          const uint64_t db = operand_desc(sm + L::V_OFF + st * L::TILE_BYTES, AC_TILE * 128 / 16);
+#pragma unroll
+          for (int k = 0; k < AC_TILE / 16; ++k)  // 16 positions: 16 rows of 128 bytes
+            mma_ts(t_o, t_w + 8 * k, db + (uint64_t)(k * (16 * 128 / 16)), id_o, i > 0 || k > 0);
+          if (t.split || w == 1) mma_commit(v_free(st));
+          mma_commit(o_done(w));
+        };
+        wait(q_full(0), segments);
+        wait(q_full(1), segments);
+        scores(0, 0);
+        if (n[1] > 0) scores(1, 0);
+#pragma unroll 1
+        for (int i = 0; i < n[0]; ++i) {
+          if (i + 1 < n[0]) scores(0, i + 1);
+          if (i + 1 < n[1]) scores(1, i + 1);
+          values(0, i);
+          if (i < n[1]) values(1, i);
+        }
+        mine += n[0];
+        other += n[1];
+        ++segments;
+      }
+    }
+    __syncwarp();
+  } else if (wid >= 8) {
+    // ------------------------------ conversion ------------------------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+    for (Walk k(a, start); k.more(a); k.next(a)) {
+      const SeqInfo& s = k.s;
+      const int n_tiles = k.n_tiles, tile0 = k.tile0, it = k.it;
+      // A pass covers 128 pieces of 16 bytes: 16 rows (D = 128) or 32 (D = 64). Eight consecutive lanes take four
+      // pieces of the same 64 columns in two neighbouring rows: their FP16 halves meet all eight 16-byte slots.
+      constexpr int PASSES = D / 32, ROWS = 64 / PASSES;
+      const int ct = tid - 256, quad = lane >> 3;
+      const int row0 = (D == 128 ? 4 * (wid - 8) + 2 * (quad >> 1) : 8 * (wid - 8) + 2 * quad) + ((lane >> 2) & 1);
+      const int blk = D == 128 ? quad & 1 : 0, piece = 4 * blk + (lane & 3);
+      const uint32_t dst = blk * (AC_TILE * 128) + row0 * 128;  // (ROWS is a multiple of 8: the swizzle is every pass's)
+      const uint32_t dst0 = dst + (((2 * (lane & 3)) ^ (row0 & 7)) << 4), dst1 = dst + (((2 * (lane & 3) + 1) ^ (row0 & 7)) << 4);
+      const int* bt = a.bt + (long long)k.seq * a.bt_stride;
+      const size_t slab = (size_t)k.head * a.npages;
+      // Two tiles' codes in registers: while one is converted the other is on its way.
+      struct Raw {
+        uint4 k[PASSES], v[PASSES];
+        float sk, sv;  // of block ct of the tile (threads 0-3)
+      } raw[2];
+      // Pages are looked up one tile ahead of the loads that need them, all at once: looked up where they are used,
+      // four dependent loads in a row made this the slowest role (1600 cycles a tile).
+      int pg[PASSES], pg_s = -1;
+      const bool scales = ct < 4;
+      auto page_at = [&](int pos) { return pos < s.len ? __ldg(bt + a.page_div.div(pos)) : -1; };
+      auto pages = [&](int r) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) pg[i] = page_at(r * AC_TILE + i * ROWS + row0);
+        if (scales) pg_s = page_at(r * AC_TILE + 16 * ct);
+      };
+      auto load = [&](Raw& w, int r) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-          const int e = i * 128 + ct, row = e / PIECES, pos = p0 + row;
-          kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-          if (pos < s.len) {
-            const int pi = a.page_div.div(pos), pg = bt[pi];
-            if ((unsigned)pg < (unsigned)a.npages) {
-              const size_t at = ((slab + pg) * a.page + (pos - pi * a.page)) * D + (e - row * PIECES) * 16;
-              kr[i] = __ldg((const uint4*)(a.q_k + at));
-              vr[i] = __ldg((const uint4*)(a.q_v + at));
-            }
-          }
+          const int pos = r * AC_TILE + i * ROWS + row0;
+          const size_t at = ((slab + pg[i]) * a.page + (pos - a.page_div.div(pos) * a.page)) * D + piece * 16;
+          const bool on = (unsigned)pg[i] < (unsigned)a.npages;  // (-1 behind the end)
+          w.k[i] = on ? __ldg((const uint4*)(a.q_k + at)) : make_uint4(0, 0, 0, 0);
+          w.v[i] = on ? __ldg((const uint4*)(a.q_v + at)) : make_uint4(0, 0, 0, 0);
         }
-        if (ct < 4) {
-          const int pos = p0 + 16 * ct;
-          sk = 0.0f;
-          sv = -1.0f;
-          if (pos < s.len) {
-            const int pg = bt[a.page_div.div(pos)];
-            if ((unsigned)pg < (unsigned)a.npages) {
-              sk = a.s_k[slab + pg];
-              sv = a.s_v[slab + pg];
-            } else {
-              atomicExch(a.status, ST_KV_PAGE);
-            }
+        if (scales) {
+          w.sk = 0.0f;
+          w.sv = -1.0f;
+          if ((unsigned)pg_s < (unsigned)a.npages) {
+            w.sk = __ldg(a.s_k + slab + pg_s);
+            w.sv = __ldg(a.s_v + slab + pg_s);
+          } else if (r * AC_TILE + 16 * ct < s.len) {
+            atomicExch(a.status, ST_KV_PAGE);
           }
         }
       };
       auto store = [&](const uint4& raw, uint32_t tile, int i) {
-        const int e = i * 128 + ct, row = e / PIECES, piece = e - row * PIECES;
         uint4 h0, h1;
         e4m3x4_to_h2(raw.x, h0.x, h0.y);
         e4m3x4_to_h2(raw.y, h0.z, h0.w);
         e4m3x4_to_h2(raw.z, h1.x, h1.y);
         e4m3x4_to_h2(raw.w, h1.z, h1.w);
-        const int blk = piece >> 2, c = (piece & 3) * 2;
-        const uint32_t base = tile + blk * (AC_TILE * 128) + row * 128;
-        // the two blocks' lanes take the halves in opposite order: all eight 16-byte slots at once
-        const uint32_t a0 = base + ((c ^ (row & 7)) << 4), a1 = base + (((c + 1) ^ (row & 7)) << 4);
-        sts128(blk ? a1 : a0, blk ? h1 : h0);
-        sts128(blk ? a0 : a1, blk ? h0 : h1);
+        sts128(tile + i * (ROWS * 128) + dst0, h0);
+        sts128(tile + i * (ROWS * 128) + dst1, h1);
       };
-      load(r0);
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int st = (it + j) & 1;
-        const uint32_t ph = (uint32_t)((it + j) >> 1) & 1u;
-        ok = __all_sync(0xffffffffu, mbar_wait(k_free(st), ph ^ 1u, a.status, ST_FLASH_TIMEOUT));
-        if (!ok) break;
+      auto convert = [&](const Raw& w, int j) {
+        const int st = (it + j) % L::STAGES;
+        const uint32_t ph = (uint32_t)((it + j) / L::STAGES) & 1u;
+        ok = ok && mbar_wait(k_free(st), ph ^ 1u, a.status, ST_FLASH_TIMEOUT);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) store(kr[i], sm + L::K_OFF + st * L::TILE_BYTES, i);
+        for (int i = 0; i < PASSES; ++i) store(w.k[i], sm + L::K_OFF + st * L::TILE_BYTES, i);
         if (ct < 4) {
           // a block without positions (behind the end, or of no page) weighs nothing: exponent -inf
-          const bool on = sv >= 0.0f;
-          const float v = fmaxf(sv, 1e-30f);
-          *(float4*)(smp + L::META_OFF + (((it + j) & 3) * 4 + ct) * 16) =
-              make_float4(on ? sk * (a.scale * AB_LOG2E) : 0.0f, on ? lg2(v) : -INFINITY, on ? 1.0f / v : 0.0f, 0.0f);
+          const bool on = w.sv >= 0.0f;
+          const float v = fmaxf(w.sv, 1e-30f);
+          *(float4*)(smp + L::META_OFF + ((it + j) % L::METAS * 4 + ct) * 16) =
+              make_float4(on ? w.sk * (a.scale * AB_LOG2E) : 0.0f, on ? lg2(v) : -INFINITY, on ? 1.0f / v : 0.0f, 0.0f);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full(st));
         ok = __all_sync(0xffffffffu, mbar_wait(v_free(st), ph ^ 1u, a.status, ST_FLASH_TIMEOUT));
-        if (!ok) break;
+        if (!ok) return;
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) store(vr[i], sm + L::V_OFF + st * L::TILE_BYTES, i);
+        for (int i = 0; i < PASSES; ++i) store(w.v[i], sm + L::V_OFF + st * L::TILE_BYTES, i);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(v_full(st));
-        if (j + 1 < n_tiles) load(r0 + j + 1);
+      };
+      pages(tile0);
+      load(raw[0], tile0);
+      pages(tile0 + 1);
+      for (int j = 0; j < n_tiles && ok; j += 2) {
+        if (j + 1 < n_tiles) {
+          load(raw[1], tile0 + j + 1);
+          pages(tile0 + j + 2);
+        }
+        convert(raw[0], j);
+        if (j + 2 < n_tiles) {
+          load(raw[0], tile0 + j + 2);
+          pages(tile0 + j + 3);
+        }
+        if (j + 1 < n_tiles) convert(raw[1], j + 1);
       }
-    } else {
-      // ------------------------------ softmax: one thread per query row ------------------------------
-      const uint32_t lane_off = (uint32_t)(wid * 32) << 16;
-      const int row = qt * AC_ROWS + tid;
-      const bool on = tid < t.rows;
+    }
+  } else {
+    // ------------------------------ softmax: one thread per query row ------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    int mine = 0;  // tiles of this warpgroup so far: phase of its barriers
+    for (Walk k(a, start); k.more(a); k.next(a)) {
+      const SeqInfo& s = k.s;
+      const RowGroup& t = k.t;
+      const int n_tiles = k.n_tiles, tile0 = k.tile0, it = k.it;
+      const int head = k.head;
+      const int w = wid >> 2, rt = tid & (AC_ROWS - 1);  // warpgroup, row of its tile
+      const uint32_t lane_off = (uint32_t)((wid & 3) * 32) << 16;
+      const uint32_t t_s = tmem + 64 * w, t_w = tmem + 128 + 32 * w, t_q = tmem + 192 + 32 * w, t_o = tmem + 256 + 128 * w;
+      const int row_in = rt + (t.split ? 0 : AC_ROWS * w), row = k.gi * AC_GROUP + row_in;
+      const bool on = row_in < t.rows;
       const int tq = on ? row / a.group : 0, hq = head * a.group + (on ? row - tq * a.group : 0);
       const int lim = !on ? 0 : (a.causal ? s.len - s.nq + tq + 1 : s.len);
-      // D = F32, A = B = F16; S: B (K) K-major; O: B (V) MN-major. By the elected thread of warp 0.
-      constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(AC_TILE >> 3) << 17) | ((uint32_t)(AC_ROWS >> 4) << 24);
-      constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(AC_ROWS >> 4) << 24);
-      auto scores = [&](int j) {
-        const int st = (it + j) & 1;
-        if (!mbar_wait(k_full(st), (uint32_t)((it + j) >> 1) & 1u, a.status, ST_FLASH_TIMEOUT)) return;
-        tc_after_sync();
-        const uint64_t db = operand_desc(sm + L::K_OFF + st * L::TILE_BYTES, 1);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_ts(t_s, t_q + 8 * k, db + (uint64_t)((k >> 2) * (AC_TILE * 128 / 16) + (k & 3) * 2), id_s, k > 0);
-        mma_commit(k_free(st));
-        mma_commit(s_full);
-        mbar_arrive(s_full);
-      };
-      auto values = [&](int j) {
-        const int st = (it + j) & 1;
-        if (!mbar_wait(v_full(st), (uint32_t)((it + j) >> 1) & 1u, a.status, ST_FLASH_TIMEOUT)) return;
-        tc_after_sync();
-        const uint64_t db = operand_desc(sm + L::V_OFF + st * L::TILE_BYTES, AC_TILE * 128 / 16);
-#pragma unroll
-        for (int k = 0; k < AC_TILE / 16; ++k)  // 16 positions: 16 rows of 128 bytes
-          mma_ts(t_o, t_s + 8 * k, db + (uint64_t)(k * (16 * 128 / 16)), id_o, j > 0 || k > 0);
-        mma_commit(v_free(st));
-        mma_commit(o_done);
-      };
-      // all four warps' stores to tensor memory are done
-      auto meet = [&]() {
-        tmem_wait_st();
+      const int all_see = a.causal ? s.len - s.nq + (row - rt) / a.group + 1 : s.len;  // positions all its rows see
+      const int j_first = t.split ? w : 0, j_step = t.split ? 2 : 1;
+      // this warp's accesses to tensor memory are done: tell the issuing thread
+      auto signal = [&](uint32_t bar) {
         tc_before_sync();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        tc_after_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
       };
       // Q to tensor memory as FP16 (BF16: by a power of two of the row's own, see attn_b8.cu)
       float scale_row = 1.0f;
@@ -385,52 +530,76 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint4 v = on ? q[8 * c + i] : make_uint4(0, 0, 0, 0);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) h[4 * i + k] = BF16 ? bf16x2_to_h2(w[k], up) : w[k];
+            for (int k = 0; k < 4; ++k) h[4 * i + k] = BF16 ? bf16x2_to_h2(x[k], up) : x[k];
           }
-          tmem_st32(t_q + 32 * c + lane_off, h);
+          if (c == 0) {
+            tmem_st32(t_q + lane_off, h);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              sts128(sm + L::Q_OFF + w * (AC_ROWS * 128) + rt * 128 + ((i ^ (rt & 7)) << 4),
+                     make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]));
+          }
         }
-        meet();
-        if (wid == 0 && ok && elect_one()) scores(0);
-        __syncwarp();
+        if (D == 128) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tmem_wait_st();
+        signal(q_full(w));
       }
-      float m = AB_NONE, l = 0.0f;
-      for (int j = 0; j < n_tiles; ++j) {
-        ok = ok && mbar_wait(s_full, (uint32_t)(it + j) & 1u, a.status, ST_FLASH_TIMEOUT);
+      // While a row has seen nothing (`bare`) its reference point is 0; the first tile with a score sets it.
+      float m = 0.0f, l = 0.0f;
+      bool bare = true;
+      for (int j = j_first; j < n_tiles; j += j_step, ++mine) {
+        ok = ok && mbar_wait(s_full(w), (uint32_t)mine & 1u, a.status, ST_FLASH_TIMEOUT);
         ok = __all_sync(0xffffffffu, ok);
         tc_after_sync();
-        float x[AC_TILE];
-        tmem_ld32(t_s + lane_off, (uint32_t*)x);
-        tmem_ld32(t_s + 32 + lane_off, (uint32_t*)x + 32);
+        union {
+          uint32_t u[AC_TILE];
+          float f[AC_TILE];
+          f32x2 p[AC_TILE / 2];
+        } x;
+        const float4* meta = (const float4*)(smp + L::META_OFF) + ((it + j) % L::METAS) * 4;
+        const int p0 = (tile0 + j) * AC_TILE;
+        float inv[4], top = -INFINITY;
+        // exponents X - m; the second half's load runs under the first half's arithmetic
+        tmem_ld32(t_s + lane_off, x.u);
         tmem_wait_ld();
-        const float4* meta = (const float4*)(smp + L::META_OFF) + ((it + j) & 3) * 4;
-        float inv[4];
-        const int p0 = (r0 + j) * AC_TILE;
-        float top = -INFINITY;
+        tmem_ld32(t_s + 32 + lane_off, x.u + 32);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+          if (b == 2) {
+            tmem_wait_ld();
+            signal(s_free(w));
+          }
           const float4 f = meta[b];
-          const float fk = f.x * scale_row;
+          const f32x2 fk = pair(f.x * scale_row), fc = pair(f.y - m);
           inv[b] = f.z;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[16 * b + i] = fmaf(x[16 * b + i], fk, f.y);
+          for (int i = 0; i < 8; ++i) x.p[8 * b + i] = fma2(x.p[8 * b + i], fk, fc);
         }
-        if (p0 + AC_TILE > t.all_see) {
+        if (p0 + AC_TILE > all_see) {
 #pragma unroll
           for (int i = 0; i < AC_TILE; ++i)
-            if (p0 + i >= lim) x[i] = -INFINITY;
+            if (p0 + i >= lim) x.f[i] = -INFINITY;
         }
 #pragma unroll
-        for (int i = 0; i < AC_TILE; ++i) top = fmaxf(top, x[i]);
-        if (__any_sync(0xffffffffu, top > m + AB_SLACK)) {
-          const float mn = top > m + AB_SLACK ? top : m, f = ex2(m - mn);
-          m = mn;
+        for (int i = 0; i < AC_TILE; i += 2) top = max3(top, x.f[i], x.f[i + 1]);
+        if (j > j_first) {  // O and the place of the weights are free again
+          ok = ok && mbar_wait(o_done(w), (uint32_t)(mine - 1) & 1u, a.status, ST_FLASH_TIMEOUT);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_after_sync();
+        }
+        const bool move = bare ? top > -INFINITY : top > AB_SLACK;
+        if (__any_sync(0xffffffffu, move)) {
+          const float by = move ? top : 0.0f, f = bare ? 0.0f : ex2(-by);  // (nothing to scale while bare)
+          m += by;
           l *= f;
-          if (j > 0) {
-            ok = ok && mbar_wait(o_done, (uint32_t)(it + j - 1) & 1u, a.status, ST_FLASH_TIMEOUT);
-            ok = __all_sync(0xffffffffu, ok);
-            tc_after_sync();
+          bare = bare && !move;
+          const f32x2 neg = pair(-by);
+#pragma unroll
+          for (int i = 0; i < AC_TILE / 2; ++i) x.p[i] = add2(x.p[i], neg);
+          if (j > j_first) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
@@ -443,33 +612,66 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
             tmem_wait_st();
           }
         }
-        uint32_t w[32];
+        uint32_t wt[32];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          float sum = 0.0f;
+          f32x2 sum = pair(0.0f);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float w0 = ex2(x[16 * b + i] - m), w1 = ex2(x[16 * b + i + 1] - m);
-            sum += w0 + w1;
-            w[8 * b + i / 2] = h2_as_u32(__floats2half2_rn(w0, w1));
+          for (int i = 0; i < 8; ++i) {
+            const float w0 = ex2(x.f[16 * b + 2 * i]), w1 = ex2(x.f[16 * b + 2 * i + 1]);
+            sum = add2(sum, pair(w0, w1));
+            wt[8 * b + i] = h2_as_u32(__floats2half2_rn(w0, w1));
           }
-          l = fmaf(sum, inv[b], l);
+          l = fmaf(lo(sum) + hi(sum), inv[b], l);
         }
-        tmem_st32(t_s + lane_off, w);
-        meet();
-        if (wid == 0 && ok && elect_one()) {
-          values(j);
-          if (j + 1 < n_tiles) scores(j + 1);
-        }
-        __syncwarp();
+        tmem_st32(t_w + lane_off, wt);
+        tmem_wait_st();
+        signal(w_full(w));
       }
+      if (bare) m = AB_NONE;
+      // the join buffer lies over Q: both warpgroups have seen their last scores
+      if (t.split) asm volatile("bar.sync 3, 256;" ::: "memory");
       // ---- the row's result, or its part of it ----
-      ok = ok && mbar_wait(o_done, (uint32_t)(it + n_tiles - 1) & 1u, a.status, ST_FLASH_TIMEOUT);
-      ok = __all_sync(0xffffffffu, ok);
-      {
+      const bool some = j_first < n_tiles;  // (the second warpgroup of a shared group of one tile has none)
+      if (some) {
+        ok = ok && mbar_wait(o_done(w), (uint32_t)(mine - 1) & 1u, a.status, ST_FLASH_TIMEOUT);
+        ok = __all_sync(0xffffffffu, ok);
         tc_after_sync();
-        const long long cta = blockIdx.x;
-        const long long row_begin = u - r0, row_end = row_begin + t.units;
+      }
+      float* join = (float*)(smp + L::JOIN_OFF);  // [row][2], then [D / 4][row][4]
+      if (t.split && w == 1) {
+        *(float2*)(join + 2 * rt) = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (some) {
+            tmem_ld32(t_o + 32 * c + lane_off, (uint32_t*)o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+          }
+          float* p = join + 2 * AC_ROWS + (8 * c * AC_ROWS + rt) * 4;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *(float4*)(p + i * AC_ROWS * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+        tc_before_sync();
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+      } else {
+        float f0 = 1.0f, f1 = 0.0f;  // factors of this warpgroup's and the other's part
+        if (t.split) {
+          asm volatile("bar.sync 3, 256;" ::: "memory");
+          const float2 other = *(const float2*)(join + 2 * rt);
+          const float ms = fmaxf(m, other.x);
+          f0 = ex2(m - ms);
+          f1 = ex2(other.x - ms);
+          m = ms;
+          l = l * f0 + other.y * f1;
+        }
+        const long long G = start.ctas, T = start.total;
+        const int cta = (int)blockIdx.x;
+        const long long row_begin = start.u_end - k.left - k.r0, row_end = row_begin + t.units;
         const int first_cta = (int)(((row_begin + 1) * G - 1) / T), last_cta = (int)((row_end * G - 1) / T);
         const bool whole = first_cta == last_cta;
         uint16_t* out = (uint16_t*)a.out + (long long)(s.q0 + tq) * a.out_stride + (size_t)hq * D;
@@ -485,20 +687,31 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
             *(uint4*)(out + 32 * c + i) = make_uint4(h[0], h[1], h[2], h[3]);
           }
         };
-        int* counters = (int*)a.chunk_ws;
-        float* parts = (float*)((uint8_t*)a.chunk_ws + counter_bytes((int)gridDim.x));
-        constexpr size_t PART = (size_t)AC_ROWS * (D + 2);
-        auto slot = [&](int k) { return parts + (size_t)(k == first_cta ? 2 * k + 1 : 2 * k) * PART; };
+        int* counter = (int*)a.chunk_ws + 2 * first_cta + w;
+        constexpr size_t PART = (size_t)AC_ROWS * (D + 2);  // floats per warpgroup
+        float* parts = (float*)((uint8_t*)a.chunk_ws + counter_bytes(2 * (int)gridDim.x)) + w * PART;
+        auto slot = [&](int k) { return parts + (size_t)(k == first_cta ? 2 * k + 1 : 2 * k) * (2 * PART); };
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
           tmem_ld32(t_o + 32 * c + lane_off, (uint32_t*)o);
           tmem_wait_ld();
+          if (t.split) {
+            const float* p = join + 2 * AC_ROWS + (8 * c * AC_ROWS + rt) * 4;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 v = *(const float4*)(p + i * AC_ROWS * 4);
+              o[4 * i] = fmaf(o[4 * i], f0, v.x * f1);
+              o[4 * i + 1] = fmaf(o[4 * i + 1], f0, v.y * f1);
+              o[4 * i + 2] = fmaf(o[4 * i + 2], f0, v.z * f1);
+              o[4 * i + 3] = fmaf(o[4 * i + 3], f0, v.w * f1);
+            }
+          }
           if (whole) {
             if (on) store32(c, o, row_norm(l));
           } else {
             // [D / 4][row][4]: consecutive rows next to each other
-            float* p = slot((int)cta) + 2 * AC_ROWS + (size_t)(8 * c) * AC_ROWS * 4 + tid * 4;
+            float* p = slot(cta) + 2 * AC_ROWS + (size_t)(8 * c * AC_ROWS + rt) * 4;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               *(float4*)(p + (size_t)i * AC_ROWS * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -508,21 +721,22 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
         if (whole) {
           if (on) finish(m, l);
         } else {
-          *(float2*)(slot((int)cta) + 2 * tid) = make_float2(m, l);
+          *(float2*)(slot(cta) + 2 * rt) = make_float2(m, l);
           __threadfence();
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (tid == 0) {
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
+          if (rt == 0) {
             const int want = last_cta - first_cta + 1;
-            is_last = atomicAdd(counters + first_cta, 1) + 1 == want;
-            if (is_last) counters[first_cta] = 0;  // as the next launch expects it
+            const bool last = atomicAdd(counter, 1) + 1 == want;
+            is_last[w] = last;
+            if (last) *counter = 0;  // as the next launch expects it
           }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (is_last && on) {
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
+          if (is_last[w] && on) {
             __threadfence();
             float ms = AB_NONE, ls = 0.0f;
-            for (int k = first_cta; k <= last_cta; ++k) ms = fmaxf(ms, __ldcg(slot(k) + 2 * tid));
+            for (int k = first_cta; k <= last_cta; ++k) ms = fmaxf(ms, __ldcg(slot(k) + 2 * rt));
             for (int k = first_cta; k <= last_cta; ++k) {
-              const float2 ml = __ldcg((const float2*)(slot(k) + 2 * tid));
+              const float2 ml = __ldcg((const float2*)(slot(k) + 2 * rt));
               ls = fmaf(ml.y, ex2(ml.x - ms), ls);
             }
             const float norm = row_norm(ls);
@@ -533,8 +747,8 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
               for (int i = 0; i < 32; ++i) v[i] = 0.0f;
 #pragma unroll 1
               for (int k = first_cta; k <= last_cta; ++k) {
-                const float* p = slot(k) + 2 * AC_ROWS + (size_t)(8 * c) * AC_ROWS * 4 + tid * 4;
-                const float f = ex2(__ldcg(slot(k) + 2 * tid) - ms);
+                const float* p = slot(k) + 2 * AC_ROWS + (size_t)(8 * c * AC_ROWS + rt) * 4;
+                const float f = ex2(__ldcg(slot(k) + 2 * rt) - ms);
                 float4 o[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[i] = __ldcg((const float4*)(p + (size_t)i * AC_ROWS * 4));
@@ -552,17 +766,7 @@ __global__ void __launch_bounds__(AC_THREADS, AC_CTAS_PER_SM) attn_b8_chunk_kern
           }
         }
       }
-    }
-    // next row tile
-    u += n_tiles;
-    it += n_tiles;
-    r0 = 0;
-    if (++qt == row_tiles(a, s)) {
-      qt = 0;
-      if (++head == a.H) {
-        head = 0;
-        if (u < u_end) s = seq_info(a, ++seq);
-      }
+      if (t.split) asm volatile("bar.sync 3, 256;" ::: "memory");  // the join buffer is free again
     }
   }
   tc_before_sync();
@@ -575,15 +779,14 @@ cudaError_t launch(const AttnB8& a, int sm_count, cudaStream_t stream) {
   auto* k = attn_b8_chunk_kernel<D, BF16>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem<D>::BYTES);
   if (e != cudaSuccess) return e;
-  k<<<AC_CTAS_PER_SM * sm_count, AC_THREADS, ChunkSmem<D>::BYTES, stream>>>(a);
+  k<<<sm_count, AC_THREADS, ChunkSmem<D>::BYTES, stream>>>(a);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 size_t attn_b8_chunk_ws_bytes(int sm_count) {
-  const int grid = AC_CTAS_PER_SM * sm_count;
-  return counter_bytes(grid) + (size_t)2 * grid * AC_ROWS * (AB_MAX_D + 2) * sizeof(float);
+  return counter_bytes(2 * sm_count) + (size_t)2 * sm_count * AC_GROUP * (AB_MAX_D + 2) * sizeof(float);
 }
 
 cudaError_t attn_b8_chunk_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaStream_t stream) {
