@@ -766,8 +766,9 @@ int w4b_kv_write_b8(const w4b_kv_b8* p, const int* slots, int T, const void* k_n
   if (T == 0) return W4B_OK;
   DeviceCtx* ctx = nullptr;
   if (int rc = get_ctx(&ctx)) return rc;
-  const KvWriteB8 a = {slots, T, k_new, v_new, k_stride, v_stride, p->page, p->npages, p->q_k, p->s_k, p->q_v, p->s_v, 1, ctx->status};
-  CUDA_TRY(kv_write_b8_launch(a, p->H, p->D, dtype == W4B_DTYPE_BF16, ctx->sm_count, (cudaStream_t)stream), "kv write b8 kernel");
+  const KvWriteB8 a = {slots, T, k_new, v_new, k_stride, v_stride, p->H, p->page, p->npages,
+                       p->q_k, p->s_k, p->q_v, p->s_v, ctx->status, 1, 1};
+  CUDA_TRY(kv_write_b8_launch(a, p->D, dtype == W4B_DTYPE_BF16, ctx->sm_count, (cudaStream_t)stream), "kv write b8 kernel");
   g_launches += 1;
   return W4B_OK;
 }

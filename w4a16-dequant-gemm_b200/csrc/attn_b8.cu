@@ -34,6 +34,7 @@ constexpr int AB_THREADS = 32 * AB_WARPS;
 constexpr int AB_CTAS_PER_SM = 4;
 constexpr int AB_STAGES = 3;
 constexpr int AB_UNIT = 64;      // positions per work unit: one block of 16 per warp
+constexpr int AB_ROW_COST = 2;   // units a row counts for besides its positions: its start, join and store take that long
 constexpr int AB_MAX_COLS = 16;  // query rows per column tile
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
@@ -65,7 +66,7 @@ template <int NC>
 __device__ __forceinline__ long long seq_units(const AttnB8& a, const SeqInfo& s, int& tiles, int& units) {
   const int rows = s.nq * a.group;
   tiles = rows < a.chunk_rows ? (rows + NC - 1) / NC : 0;  // the others are the chunk kernel's
-  units = max(1, (s.len + AB_UNIT - 1) / AB_UNIT);
+  units = max(1, (s.len + AB_UNIT - 1) / AB_UNIT) + AB_ROW_COST;
   return (long long)a.H * tiles * units;
 }
 
@@ -162,8 +163,15 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
       continue;
     }
     // row = (head, column tile) of the sequence; units [r0, r1) of it are this CTA's
-    const int row = (int)(off / units), r0 = (int)(off - (long long)row * units);
-    const int r1 = (int)min((long long)units, r0 + (u_end - u));
+    const int row = (int)(off / units), at = (int)(off - (long long)row * units);
+    const int step = (int)min((long long)(units - at), u_end - u);
+    // (the first AB_ROW_COST units of a row stand for no positions)
+    const int r0 = max(0, at - AB_ROW_COST), r1 = at + step - AB_ROW_COST;
+    if (r1 <= 0) {
+      u += step;
+      off += step;
+      continue;
+    }
     const int head = row / tiles, tile = row - head * tiles;
     const int rows = min(NC, s.nq * a.group - tile * NC);   // query rows in this tile
     const int tq0 = tile * NC / a.group;                      // first and last query token of the tile
@@ -173,6 +181,46 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     const int p_begin = r0 * AB_UNIT, p_end = min(r1 * AB_UNIT, end);
     const int nblocks = p_end > p_begin ? (p_end - p_begin + 15) / 16 : 0;
     const int mine_n = nblocks > wid ? (nblocks - wid + AB_WARPS - 1) / AB_WARPS : 0;
+
+    // ---- the ring ------------------------------------------------------------------------------------------------
+    const int* bt = a.bt + (long long)seq * a.bt_stride;
+    const size_t slab = (size_t)head * a.npages;
+    auto position = [&](int j) { return p_begin + (wid + j * AB_WARPS) * 16; };
+    auto page_of = [&](int j) { return j < mine_n ? bt[a.page_div.div(position(j))] : 0; };
+    auto issue = [&](int j, int pg) {
+      const uint32_t st = ring + (j % AB_STAGES) * C::STAGE;
+      if (j < mine_n) {
+        const int p0 = position(j);
+        const bool good = (unsigned)pg < (unsigned)a.npages;
+        const size_t r = (slab + (good ? pg : 0)) * a.page + (p0 - a.page_div.div(p0) * a.page);
+        const uint8_t* ks = a.q_k + r * D;
+        const uint8_t* vs = a.q_v + r * D;
+#pragma unroll
+        for (int i = 0; i < C::SIDE / 512; ++i) {
+          const int e = i * 32 + lane, rr = e / C::PIECES, jj = e - rr * C::PIECES;
+          const bool on = good && p0 + rr < s.len;
+          cp_async16_zfill(st + C::piece(rr, jj), ks + (on ? e * 16 : 0), on);
+          cp_async16_zfill(st + C::SIDE + C::piece(rr, jj), vs + (on ? e * 16 : 0), on);
+        }
+        if (lane < 2) {
+          const float* sc = (lane == 0 ? a.s_k : a.s_v) + slab + (good ? pg : 0);
+          if (good) {
+            cp_async<4>(st + 2 * C::SIDE + 4 * lane, sc);
+          } else {
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * C::SIDE + 4 * lane), "f"(-1.0f) : "memory");
+            if (lane == 0) atomicExch(a.status, ST_KV_PAGE);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    int pg_next = page_of(0);
+#pragma unroll
+    for (int j = 0; j < AB_STAGES - 1; ++j) {
+      const int pg = pg_next;
+      pg_next = page_of(j + 1);
+      issue(j, pg);
+    }
 
     // ---- query rows as operand registers: lane (g, c) holds row g, dims 16 i + 4 c .. + 3 ----------------------
     uint32_t qf[NT][C::KSTEPS][2];
@@ -237,46 +285,6 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
         m[t][j] = AB_NONE;
         l[t][j] = 0.0f;
       }
-
-    // ---- the ring ------------------------------------------------------------------------------------------------
-    const int* bt = a.bt + (long long)seq * a.bt_stride;
-    const size_t slab = (size_t)head * a.npages;
-    auto position = [&](int j) { return p_begin + (wid + j * AB_WARPS) * 16; };
-    auto page_of = [&](int j) { return j < mine_n ? bt[a.page_div.div(position(j))] : 0; };
-    auto issue = [&](int j, int pg) {
-      const uint32_t st = ring + (j % AB_STAGES) * C::STAGE;
-      if (j < mine_n) {
-        const int p0 = position(j);
-        const bool good = (unsigned)pg < (unsigned)a.npages;
-        const size_t r = (slab + (good ? pg : 0)) * a.page + (p0 - a.page_div.div(p0) * a.page);
-        const uint8_t* ks = a.q_k + r * D;
-        const uint8_t* vs = a.q_v + r * D;
-#pragma unroll
-        for (int i = 0; i < C::SIDE / 512; ++i) {
-          const int e = i * 32 + lane, rr = e / C::PIECES, jj = e - rr * C::PIECES;
-          const bool on = good && p0 + rr < s.len;
-          cp_async16_zfill(st + C::piece(rr, jj), ks + (on ? e * 16 : 0), on);
-          cp_async16_zfill(st + C::SIDE + C::piece(rr, jj), vs + (on ? e * 16 : 0), on);
-        }
-        if (lane < 2) {
-          const float* sc = (lane == 0 ? a.s_k : a.s_v) + slab + (good ? pg : 0);
-          if (good) {
-            cp_async<4>(st + 2 * C::SIDE + 4 * lane, sc);
-          } else {
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * C::SIDE + 4 * lane), "f"(-1.0f) : "memory");
-            if (lane == 0) atomicExch(a.status, ST_KV_PAGE);
-          }
-        }
-      }
-      cp_async_commit();
-    };
-    int pg_next = page_of(0);
-#pragma unroll
-    for (int j = 0; j < AB_STAGES - 1; ++j) {
-      const int pg = pg_next;
-      pg_next = page_of(j + 1);
-      issue(j, pg);
-    }
 
     for (int j = 0; j < mine_n; ++j) {
       cp_async_wait<AB_STAGES - 2>();
@@ -398,8 +406,8 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     __syncthreads();
 
     // where the row begins and ends among the CTAs
-    const long long row_begin = u - r0, row_end = row_begin + units;
-    const bool whole = r0 == 0 && r1 == units;
+    const long long row_begin = u - at + AB_ROW_COST, row_end = u - at + units;
+    const bool whole = r0 == 0 && r1 == units - AB_ROW_COST;
     const int first_cta = (int)(((row_begin + 1) * G - 1) / T), last_cta = (int)((row_end * G - 1) / T);
     constexpr int LANES = D / 8;  // threads per column
     auto store_row = [&](int n, int d, const float v[8], float ms, float ls) {
@@ -463,34 +471,52 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
           const int n = e / LANES, d = (e - n * LANES) * 8;
           if (n >= rows) continue;
           auto slot = [&](int k) { return parts + (size_t)(k == first_cta ? 2 * k + 1 : 2 * k) * C::PART; };
+          // one pass, four parts in flight, in CTA order
           float ms = AB_NONE, ls = 0.0f, v[8];
-          for (int k = first_cta; k <= last_cta; ++k) ms = fmaxf(ms, __ldcg(slot(k) + 2 * n));
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-#pragma unroll 4
-          for (int k = first_cta; k <= last_cta; ++k) {
-            const float* src = slot(k);
-            const float2 st = __ldcg((const float2*)(src + 2 * n));
-            const float4 o0 = __ldcg((const float4*)(src + 2 * NC + n * D + d));
-            const float4 o1 = __ldcg((const float4*)(src + 2 * NC + n * D + d) + 1);
-            const float f = ex2(st.x - ms);
-            ls = fmaf(st.y, f, ls);
-            v[0] = fmaf(o0.x, f, v[0]);
-            v[1] = fmaf(o0.y, f, v[1]);
-            v[2] = fmaf(o0.z, f, v[2]);
-            v[3] = fmaf(o0.w, f, v[3]);
-            v[4] = fmaf(o1.x, f, v[4]);
-            v[5] = fmaf(o1.y, f, v[5]);
-            v[6] = fmaf(o1.z, f, v[6]);
-            v[7] = fmaf(o1.w, f, v[7]);
+          for (int k = first_cta; k <= last_cta; k += 4) {
+            float2 st[4];
+            float4 o[4][2];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const float* src = slot(min(k + b, last_cta));
+              st[b] = __ldcg((const float2*)(src + 2 * n));
+              o[b][0] = __ldcg((const float4*)(src + 2 * NC + n * D + d));
+              o[b][1] = __ldcg((const float4*)(src + 2 * NC + n * D + d) + 1);
+            }
+            float mn = ms;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              if (k + b > last_cta) st[b] = make_float2(AB_NONE, 0.0f);
+              mn = fmaxf(mn, st[b].x);
+            }
+            const float f0 = ex2(ms - mn);
+            ms = mn;
+            ls *= f0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= f0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const float f = k + b > last_cta ? 0.0f : ex2(st[b].x - ms);
+              ls = fmaf(st[b].y, f, ls);
+              v[0] = fmaf(o[b][0].x, f, v[0]);
+              v[1] = fmaf(o[b][0].y, f, v[1]);
+              v[2] = fmaf(o[b][0].z, f, v[2]);
+              v[3] = fmaf(o[b][0].w, f, v[3]);
+              v[4] = fmaf(o[b][1].x, f, v[4]);
+              v[5] = fmaf(o[b][1].y, f, v[5]);
+              v[6] = fmaf(o[b][1].z, f, v[6]);
+              v[7] = fmaf(o[b][1].w, f, v[7]);
+            }
           }
           store_row(n, d, v, ms, ls);
         }
       }
     }
     __syncthreads();  // the merge buffer becomes the ring again
-    u += r1 - r0;
-    off += r1 - r0;
+    u += step;
+    off += step;
   }
 }
 

@@ -11,9 +11,13 @@
 // loses no precision by it, its step being relative. A row with a value that is not finite is written as zeros and
 // reported through the status word, like the other quantizers do.
 //
-// One CTA per (run, head, side): memory-bound, every value is read once (16-byte loads, kept in registers between the
-// maximum and the rounding) and every code written once. |x| of FP16 and BF16 order like their bit patterns, so the
-// maximum is taken on packed 16-bit integers. A CTA looks for the runs that begin in its window of tokens.
+// Memory-bound: every value is read once (16-byte loads, kept in registers between the maximum and the rounding) and
+// every code written once. |x| of FP16 and BF16 order like their bit patterns, so the maximum is taken on packed 16-bit
+// integers. A CTA looks for the runs that begin in its window of tokens and takes some of the 2 H (side, head) items of
+// each: finding a run is two dependent reads of the slot map, which a long step's CTAs share between several items.
+// Measured: 64 single tokens, 8 heads of 128, FP16: 3.3 us; 17,417 tokens, 8 heads of 128 out of rows of 12 KB, BF16:
+// 29.2 us = 3.7 TB/s, 0.56 of the measured copy rate (39.6 us with a CTA for every run and item). What is left there
+// are the instructions around each run and item; loads one item ahead cost more registers than they hid.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -23,7 +27,8 @@
 namespace w4b {
 namespace {
 
-constexpr int KW_HELD = 4;            // 8-value pieces a thread keeps in registers
+constexpr int KW_HELD = 8;            // 8-value pieces a thread keeps in registers (4: 30.4 us where 8 take 29.2)
+constexpr int KW_BLOCKS = 2;          // CTAs of 512 threads per SM: 64 registers a thread
 constexpr int KW_MIN_EXP = -60, KW_MAX_EXP = 60;
 
 template <bool BF16>
@@ -32,24 +37,26 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   return __half22float2(u32_as_h2(v));
 }
 
-__device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) { return __vmaxu2(a, b & 0x7FFF7FFFu); }
-
-// 8 values times / over the scale to 8 codes
+// 8 values over the scale to 8 codes; a scale that is a power of two (every one this kernel makes) is a multiplication
 template <bool BF16>
-__device__ __forceinline__ uint2 encode8(uint4 v, float s, float inv, bool pow2) {
+__device__ __forceinline__ uint2 encode8(uint4 v, float inv) {
   const uint32_t in[4] = {v.x, v.y, v.z, v.w};
   uint32_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 f = unpack2<BF16>(in[i]);
-    if (pow2) {
-      f.x *= inv;
-      f.y *= inv;
-    } else {
-      f.x = __fdiv_rn(f.x, s);
-      f.y = __fdiv_rn(f.y, s);
-    }
-    h[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+    const float2 f = unpack2<BF16>(in[i]);
+    h[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x * inv, f.y * inv), __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+template <bool BF16>
+__device__ __noinline__ uint2 encode8_div(uint4 v, float s) {
+  const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+  uint32_t h[4];
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<BF16>(in[i]);
+    h[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f.x, s), __fdiv_rn(f.y, s)), __NV_SATFINITE, __NV_E4M3);
   }
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
@@ -67,24 +74,31 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
 }
 
 template <bool BF16, int D>
-__global__ void kv_write_b8_kernel(const KvWriteB8 a) {
+__global__ void __launch_bounds__(512, KW_BLOCKS) kv_write_b8_kernel(const KvWriteB8 a) {
   constexpr int LPR = D / 8;  // lanes per row
-  __shared__ uint32_t wmax[16];
+  __shared__ uint32_t wmax[2][16];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, nthreads = blockDim.x;
-  const int h = (int)blockIdx.y;
-  const bool v_side = blockIdx.z != 0;
-  const uint16_t* x = (const uint16_t*)(v_side ? a.v_new : a.k_new) + (size_t)h * D;
-  const long long xs = v_side ? a.v_stride : a.k_stride;
   const long long rows = (long long)a.npages * a.page;
-  uint8_t* codes = (v_side ? a.q_v : a.q_k) + (size_t)h * rows * D;
-  float* scales = (v_side ? a.s_v : a.s_k) + (size_t)h * a.npages;
   const uint32_t inf_bits = BF16 ? 0x7F80u : 0x7C00u;
 
-  // tokens that head a run, 32 at a time
-  const int t_begin = (int)blockIdx.x * a.window, t_end = min(t_begin + a.window, a.T);
-  for (int t0 = t_begin; t0 < t_end; t0 += 32) {
-    uint32_t heads = 0;
-    {
+  // this CTA's tokens and items (sides and heads; the CTAs of neighbouring items are launched together, since they
+  // read the same tokens' rows)
+  const int groups = (2 * a.H + a.items - 1) / a.items, win = (int)(blockIdx.x / groups);
+  const int item0 = (int)(blockIdx.x - (unsigned)win * groups) * a.items, item1 = min(item0 + a.items, 2 * a.H);
+  const int t_begin = win * a.window, t_end = (int)min((long long)t_begin + a.window, (long long)a.T);
+
+  struct Task {
+    int t, n;     // tokens t .. t + n - 1: a run
+    int p, row0;  // its page, the row it starts at
+    int item;     // < H: keys of head `item`; else values of head item - H
+  };
+  int t0 = t_begin - 32;
+  uint32_t heads = 0;  // tokens t0 + bit that head a run
+  auto advance = [&](Task& k) {  // the next item of the run, or the first of the next run; the same in every thread
+    if (k.n > 0 && ++k.item < item1) return true;
+    while (heads == 0) {
+      t0 += 32;
+      if (t0 >= t_end) return false;
       const int t = t0 + lane;
       bool head = false, wrong = false;
       if (t < t_end) {
@@ -100,96 +114,109 @@ __global__ void kv_write_b8_kernel(const KvWriteB8 a) {
       if (wrong && wid == 0) atomicExch(a.status, ST_KV_WRITE_SLOT);
       heads = __ballot_sync(0xffffffffu, head);
     }
-    while (heads != 0) {
-      const int t = t0 + __ffs(heads) - 1;
-      heads &= heads - 1;
-      const int slot = a.slots[t];
-      const int p = slot / a.page, row0 = slot - p * a.page;
-      // the run: tokens t .. t + n - 1 in slots slot, slot + 1, ... of the page
-      int n = 1;
-      const int most = min(a.page - row0, a.T - t);
-      while (n < most) {  // every warp by itself
-        const int j = n + lane;
-        const uint32_t on = __ballot_sync(0xffffffffu, j < most && a.slots[t + j] == slot + j);
-        n += on == 0xffffffffu ? 32 : __ffs(~on) - 1;
-        if (on != 0xffffffffu) break;
-      }
-      const int pieces = n * LPR;
-      uint4 held[KW_HELD];
-      uint32_t top = 0;
-      bool finite = true;
-      // rows with a value that is not finite count as zeros
-      auto row_of = [&](int i) -> uint4 {
-        const uint16_t* src = x + (long long)(t + i / LPR) * xs + (i % LPR) * 8;
-        return i < pieces ? *(const uint4*)src : make_uint4(0, 0, 0, 0);
-      };
-      auto row_max = [&](uint4& v) {
-        uint32_t m = abs_max2(abs_max2(abs_max2(abs_max2(0u, v.x), v.y), v.z), v.w);
-        m = max(m & 0xFFFFu, m >> 16);
+    k.t = t0 + __ffs(heads) - 1;
+    heads &= heads - 1;
+    const int slot = a.slots[k.t];
+    k.p = slot / a.page;
+    k.row0 = slot - k.p * a.page;
+    k.item = item0;
+    k.n = 1;
+    const int most = min(a.page - k.row0, a.T - k.t);
+    while (k.n < most) {
+      const int j = k.n + lane;
+      const uint32_t on = __ballot_sync(0xffffffffu, j < most && a.slots[k.t + j] == slot + j);
+      k.n += on == 0xffffffffu ? 32 : __ffs(~on) - 1;
+      if (on != 0xffffffffu) break;
+    }
+    return true;
+  };
+  Task k = {0, 0, 0, 0, 0};
+  for (int turn = 0; advance(k); turn ^= 1) {
+    const bool v_side = k.item >= a.H;
+    const int h = v_side ? k.item - a.H : k.item, pieces = k.n * LPR;
+    // this thread's pieces: i * nthreads + tid, row (i * nthreads + tid) / LPR of the run
+    const long long stride = v_side ? a.v_stride : a.k_stride;
+    const uint16_t* x = (const uint16_t*)(v_side ? a.v_new : a.k_new) + (size_t)h * D + (long long)(k.t + tid / LPR) * stride +
+                        (tid % LPR) * 8;
+    const long long pass = (long long)(nthreads / LPR) * stride;
+    float* scale = (v_side ? a.s_v : a.s_k) + (size_t)h * a.npages + k.p;
+    uint4 held[KW_HELD];
 #pragma unroll
-        for (int d = LPR / 2; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-        if (m >= inf_bits) {
+    for (int i = 0; i < KW_HELD; ++i)
+      held[i] = i * nthreads + tid < pieces ? *(const uint4*)(x + i * pass) : make_uint4(0, 0, 0, 0);
+    const float old = *scale;
+    uint32_t top = 0;
+    bool finite = true;
+    auto row_max = [&](uint4& v) {  // a row with a value that is not finite counts as zeros
+      uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+      const bool bad = (m & 0xFFFFu) >= inf_bits || (m >> 16) >= inf_bits;
+      if (__any_sync(0xffffffffu, bad)) {
+        bool row = bad;
+#pragma unroll
+        for (int d = LPR / 2; d > 0; d >>= 1) row = __shfl_xor_sync(0xffffffffu, (int)row, d) || row;
+        if (row) {
           finite = false;
           v = make_uint4(0, 0, 0, 0);
           m = 0;
         }
-        return m;
-      };
-#pragma unroll
-      for (int k = 0; k < KW_HELD; ++k) {
-        held[k] = make_uint4(0, 0, 0, 0);
-        if (k * nthreads < pieces) held[k] = row_of(k * nthreads + tid);
       }
-      const float old = scales[p];
+      return m;
+    };
 #pragma unroll
-      for (int k = 0; k < KW_HELD; ++k)
-        if (k * nthreads < pieces) top = max(top, row_max(held[k]));
-      for (int k = KW_HELD; k * nthreads < pieces; ++k) {
-        uint4 v = row_of(k * nthreads + tid);
-        top = max(top, row_max(v));
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) wmax[wid] = top;
-      __syncthreads();
-      for (int w = 0; w < nthreads / 32; ++w) top = max(top, wmax[w]);
-      __syncthreads();  // wmax is free for the next run; scales[p] has been read by all
-      const float amax = BF16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
+    for (int i = 0; i < KW_HELD; ++i)
+      if (i * nthreads < pieces) top = __vmaxu2(top, row_max(held[i]));
+#pragma unroll 1
+    for (int i = KW_HELD; i * nthreads < pieces; ++i) {  // pages larger than the registers: read twice
+      uint4 v = i * nthreads + tid < pieces ? *(const uint4*)(x + i * pass) : make_uint4(0, 0, 0, 0);
+      top = __vmaxu2(top, row_max(v));
+    }
+    top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+    if (lane == 0) wmax[turn][wid] = top;
+    __syncthreads();  // (and the scale has been read by all)
+    for (int w = 0; w < nthreads / 32; ++w) top = max(top, wmax[turn][w]);
+    const float amax = BF16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
 
-      float s = old;
-      bool moved = false;
-      if (row0 == 0 || !(amax <= 448.0f * old)) {
-        int e = KW_MIN_EXP;
-        if (amax > 0.0f) {
-          int b;
-          const float m = frexpf(amax, &b);
-          e = b - 9 + (m > 0.875f ? 1 : 0);  // 448 = 0.875 * 2^9
-          if (e > KW_MAX_EXP && tid == 0) atomicExch(a.status, ST_QUANT_INVALID);
-          e = min(max(e, KW_MIN_EXP), KW_MAX_EXP);
-        }
-        s = __uint_as_float((uint32_t)(e + 127) << 23);
-        moved = row0 > 0;
+    float s = old;
+    bool moved = false;
+    if (k.row0 == 0 || !(amax <= 448.0f * old)) {
+      int e = KW_MIN_EXP;
+      if (amax > 0.0f) {
+        int b;
+        const float m = frexpf(amax, &b);
+        e = b - 9 + (m > 0.875f ? 1 : 0);  // 448 = 0.875 * 2^9
+        if (e > KW_MAX_EXP && tid == 0) atomicExch(a.status, ST_QUANT_INVALID);
+        e = min(max(e, KW_MIN_EXP), KW_MAX_EXP);
       }
-      if (tid == 0 && s != old) scales[p] = s;
-      if (!finite && (lane % LPR) == 0) atomicExch(a.status, ST_QUANT_INVALID);
-      uint8_t* page_codes = codes + (size_t)p * a.page * D;
-      if (moved) {
-        const float ratio = old / s;
-        uint32_t* w = (uint32_t*)page_codes;
-        for (int i = tid; i < row0 * (D / 4); i += nthreads) w[i] = recode4(w[i], ratio);
-      }
-      const bool pow2 = (__float_as_uint(s) & 0x007FFFFFu) == 0;
+      s = __uint_as_float((uint32_t)(e + 127) << 23);
+      moved = k.row0 > 0;
+    }
+    if (tid == 0 && s != old) *scale = s;
+    if (!finite && (lane % LPR) == 0) atomicExch(a.status, ST_QUANT_INVALID);
+    uint8_t* page_codes = (v_side ? a.q_v : a.q_k) + ((size_t)h * rows + (size_t)k.p * a.page) * D;
+    if (moved) {
+      const float ratio = old / s;
+      uint32_t* w = (uint32_t*)page_codes;
+#pragma unroll 1
+      for (int i = tid; i < k.row0 * (D / 4); i += nthreads) w[i] = recode4(w[i], ratio);
+    }
+    uint2* dst = (uint2*)(page_codes + (size_t)k.row0 * D) + tid;
+    if ((__float_as_uint(s) & 0x007FFFFFu) == 0) {
       const float inv = 1.0f / s;
-      uint2* dst = (uint2*)(page_codes + (size_t)row0 * D);
 #pragma unroll
-      for (int k = 0; k < KW_HELD; ++k) {
-        const int i = k * nthreads + tid;
-        if (i < pieces) dst[i] = encode8<BF16>(held[k], s, inv, pow2);
-      }
-      for (int k = KW_HELD; k * nthreads < pieces; ++k) {
-        const int i = k * nthreads + tid;
-        uint4 v = row_of(i);
+      for (int i = 0; i < KW_HELD; ++i)
+        if (i * nthreads + tid < pieces) dst[i * nthreads] = encode8<BF16>(held[i], inv);
+#pragma unroll 1
+      for (int i = KW_HELD; i * nthreads < pieces; ++i) {
+        uint4 v = i * nthreads + tid < pieces ? *(const uint4*)(x + i * pass) : make_uint4(0, 0, 0, 0);
         row_max(v);
-        if (i < pieces) dst[i] = encode8<BF16>(v, s, inv, pow2);
+        if (i * nthreads + tid < pieces) dst[i * nthreads] = encode8<BF16>(v, inv);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i * nthreads < pieces; ++i) {
+        uint4 v = i * nthreads + tid < pieces ? *(const uint4*)(x + i * pass) : make_uint4(0, 0, 0, 0);
+        row_max(v);
+        if (i * nthreads + tid < pieces) dst[i * nthreads] = encode8_div<BF16>(v, s);
       }
     }
   }
@@ -197,17 +224,22 @@ __global__ void kv_write_b8_kernel(const KvWriteB8 a) {
 
 }  // namespace
 
-cudaError_t kv_write_b8_launch(const KvWriteB8& args, int H, int D, int bf16, int sm_count, cudaStream_t stream) {
+cudaError_t kv_write_b8_launch(const KvWriteB8& args, int D, int bf16, int sm_count, cudaStream_t stream) {
   KvWriteB8 a = args;
   // threads: a full page's pieces, KW_HELD per thread
   int threads = a.page * (D / 8) / KW_HELD;
-  threads = threads < 64 ? 64 : (threads > 512 ? 512 : (threads + 31) / 32 * 32);
-  // window: single-token runs (a decode step) want a CTA each; prompt steps want about a page per CTA, or most of the
-  // grid would only find that its token heads no run. About two waves of CTAs decide between the two.
-  const long long items = (long long)a.T * H * 2, grid = 2LL * sm_count * (2048 / threads);
-  long long w = items / grid;
-  a.window = (int)(w < 1 ? 1 : (w > a.page ? a.page : w));
-  const dim3 g((unsigned)((a.T + a.window - 1) / a.window), (unsigned)H, 2);
+  threads = threads < 32 ? 32 : (threads > 512 ? 512 : (threads + 31) / 32 * 32);
+  // One wave of CTAs: single-token runs (a decode step) get a CTA for each item; longer steps first wider windows, up
+  // to a page (a narrower one would mostly find that its token heads no run), then several items per CTA.
+  const long long wave = (long long)sm_count * (KW_BLOCKS * 512 / threads), all = 2LL * a.H * a.T;
+  const long long w = (all + wave - 1) / wave;
+  a.window = (int)(w > a.page ? a.page : w);
+  const long long windows = (a.T + (long long)a.window - 1) / a.window;
+  long long groups = wave / windows;
+  groups = groups < 1 ? 1 : (groups > 2 * a.H ? 2 * a.H : groups);
+  a.items = (int)((2 * a.H + groups - 1) / groups);
+  const long long grid = windows * ((2 * a.H + a.items - 1) / a.items);
+  const dim3 g((unsigned)grid);
   if (D == 128) {
     if (bf16) kv_write_b8_kernel<true, 128><<<g, threads, 0, stream>>>(a);
     else kv_write_b8_kernel<false, 128><<<g, threads, 0, stream>>>(a);

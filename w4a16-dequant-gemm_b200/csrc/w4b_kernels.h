@@ -69,15 +69,15 @@ struct KvWriteB8 {
   const void* k_new;  // FP16 or BF16, a row of H * D values every k_stride values
   const void* v_new;
   long long k_stride, v_stride;
-  int page, npages;
+  int H, page, npages;
   uint8_t* q_k;
   float* s_k;
   uint8_t* q_v;
   float* s_v;
-  int window;  // tokens a CTA looks through for runs to write (set by the launcher)
   int* status;
+  int window, items;  // tokens a CTA looks through, (side, head) items it takes (set by the launcher)
 };
-cudaError_t kv_write_b8_launch(const KvWriteB8& a, int H, int D, int bf16, int sm_count, cudaStream_t stream);
+cudaError_t kv_write_b8_launch(const KvWriteB8& a, int D, int bf16, int sm_count, cudaStream_t stream);
 
 // ---- attn_b8.cu, attn_b8_chunk.cu ---------------------------------------------
 // n / d for 0 <= n < 2^31 by a multiplication: with m = floor(2^(31 + s) / d) + 1, s = ceil(log2 d), the error
