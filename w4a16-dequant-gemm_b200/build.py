@@ -10,11 +10,13 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libw4b200.so")
+FASTCALL = os.path.join(LIB_DIR, "_w4b_fastcall.so")  # CPython binding of the per-step entries (csrc/fastcall.cpp)
 SOURCES = ["abi.cu", "dequant.cu", "gemm_generic.cu", "gemm_stream.cu", "gemm_noalloc.cu", "gemm_tensor.cu", "attn_flash.cu", "attn_mma.cu", "peer_gather.cu", "quantize.cu", "relayout.cu",
            "page_tables.cu", "kv_write_b8.cu", "attn_b8.cu", "attn_b8_chunk.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -22,9 +24,9 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
 
 
 def _stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(FASTCALL):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(FASTCALL))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(os.path.dirname(HERE), "include", "w4b_abi.h"))
     return any(os.path.getmtime(d) > t for d in deps)
@@ -42,6 +44,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
     if verbose:
         print(r.stderr)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"],
+           os.path.join(CSRC, "fastcall.cpp"), "-o", FASTCALL, "-L" + LIB_DIR, "-l:libw4b200.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
     return LIB
 
 

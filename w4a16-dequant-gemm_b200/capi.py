@@ -11,6 +11,7 @@ There is no CPU fallback: without the compiled library the import fails.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 from dataclasses import dataclass
 from typing import Optional
@@ -119,6 +120,19 @@ def _load():
 
 
 lib = _load()
+
+
+def _load_fastcall():
+    # the same library through CPython's call protocol, for the entries a serving loop calls every step
+    if not os.path.exists(_build.FASTCALL):
+        raise ImportError(f"{_build.FASTCALL} is missing: build it with `python w4a16-dequant-gemm_b200/build.py`")
+    spec = importlib.util.spec_from_file_location("_w4b_fastcall", _build.FASTCALL)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+_fast = _load_fastcall()
 
 
 def _check(rc: int):
@@ -334,14 +348,19 @@ def page_tables(cached, fresh, nseq, page, npages, free_pages, nfree, taken_in, 
     """Block tables, lengths, token offsets and the slot / position of every token of a step, from the requests'
     cached[i] positions and fresh[i] new tokens. All arrays are device int32; new pages come from
     free_pages[taken_in[0]:]. seq_lens may be cached and taken_out taken_in."""
-    _check(lib.w4b_page_tables(cached, fresh, nseq, page, npages, free_pages, nfree, taken_in, taken_out, bt, bt_stride,
-                               seq_lens, q_offsets, slots, positions, max_tokens, stream))
+    rc = _fast.page_tables(cached, fresh, nseq, page, npages, free_pages, nfree, taken_in, taken_out, bt, bt_stride,
+                           seq_lens, q_offsets, slots, positions, max_tokens, stream)
+    if rc:
+        _check(rc)
 
 
 def kv_write_b8(p: DeviceKVB8, slots, T, k_new, v_new, k_stride, v_stride, dtype=DTYPE_F16, stream=None):
     """Quantises T tokens' keys and values (H*D FP16 / BF16 values every k_stride / v_stride values) into the rows
     slots[t] of the cache; pages get or raise their scale as needed. slots[t] == -1 skips a token."""
-    _check(lib.w4b_kv_write_b8(C.byref(p._c()), slots, T, k_new, v_new, k_stride, v_stride, dtype, stream))
+    rc = _fast.kv_write_b8(p.H, p.D, p.page, p.npages, p.q_k, p.s_k, p.q_v, p.s_v, slots, T, k_new, v_new, k_stride,
+                           v_stride, dtype, stream)
+    if rc:
+        _check(rc)
 
 
 def attention_b8_workspace(max_q, Hq, H) -> int:
@@ -359,9 +378,12 @@ def attention_b8_paged(p: DeviceKVB8, bt, bt_stride, seq_lens, q_offsets, nseq, 
     sequence i's query tokens (None: one each); causal: they are its last positions; otherwise every token sees all
     seq_lens[i] positions (cross attention). scale defaults to D ** -0.5. Calls that may overlap, captured ones
     among them, need a zero-filled workspace each; without one they share library scratch."""
-    _check(lib.w4b_attn_b8_paged(C.byref(p._c()), bt, bt_stride, seq_lens, q_offsets, nseq, max_q, max_seq_len, q,
-                                 q_stride, Hq, dtype, max(p.D, 1) ** -0.5 if scale is None else scale, int(causal), out,
-                                 out_stride, lse, workspace, workspace_bytes, stream))
+    rc = _fast.attn_b8_paged(p.H, p.D, p.page, p.npages, p.q_k, p.s_k, p.q_v, p.s_v, bt, bt_stride, seq_lens, q_offsets,
+                             nseq, max_q, max_seq_len, q, q_stride, Hq, dtype,
+                             max(p.D, 1) ** -0.5 if scale is None else scale, causal, out, out_stride, lse, workspace,
+                             workspace_bytes, stream)
+    if rc:
+        _check(rc)
 
 
 # ---- offline re-layout: the same matrix zero-extended along K (no counterpart in the reference) ----

@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
   const long long G = T < (long long)gridDim.x ? T : (long long)gridDim.x;
   const long long cta = blockIdx.x;
   if (cta >= G) return;
-  const long long u_begin = T * cta / G, u_end = T * (cta + 1) / G;
+  const long long u_begin = range_begin(T, cta, G), u_end = range_begin(T, cta + 1, G);
   if (u_begin >= before && u_begin < before + mine) {
     long long off = u_begin - before;
     int i = i_begin;
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
       continue;
     }
     // row = (head, column tile) of the sequence; units [r0, r1) of it are this CTA's
-    const int row = (int)(off / units), at = (int)(off - (long long)row * units);
+    const int row = off < 0x7FFFFFFF ? (int)off / units : (int)(off / units), at = (int)(off - (long long)row * units);
     const int step = (int)min((long long)(units - at), u_end - u);
     // (the first AB_ROW_COST units of a row stand for no positions)
     const int r0 = max(0, at - AB_ROW_COST), r1 = at + step - AB_ROW_COST;
@@ -406,9 +406,9 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     __syncthreads();
 
     // where the row begins and ends among the CTAs
-    const long long row_begin = u - at + AB_ROW_COST, row_end = u - at + units;
     const bool whole = r0 == 0 && r1 == units - AB_ROW_COST;
-    const int first_cta = (int)(((row_begin + 1) * G - 1) / T), last_cta = (int)((row_end * G - 1) / T);
+    const int first_cta = whole ? (int)cta : unit_owner(u - at + AB_ROW_COST, T, G);
+    const int last_cta = whole ? (int)cta : unit_owner(u - at + units - 1, T, G);
     constexpr int LANES = D / 8;  // threads per column
     auto store_row = [&](int n, int d, const float v[8], float ms, float ls) {
       // d: first of eight dims; v unnormalised
@@ -525,10 +525,9 @@ int attn_b8_grid(int sm_count) { return AB_CTAS_PER_SM * sm_count; }
 template <int D, int NT, bool BF16>
 cudaError_t launch(const AttnB8& a, int sm_count, cudaStream_t stream) {
   using C = AttnB8Kernel<D, NT, BF16>;
-  auto* k = attn_b8_kernel<D, NT, BF16>;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  const cudaError_t e = opt_in_smem<attn_b8_kernel<D, NT, BF16>>(C::SMEM);
   if (e != cudaSuccess) return e;
-  k<<<attn_b8_grid(sm_count), AB_THREADS, C::SMEM, stream>>>(a);
+  attn_b8_kernel<D, NT, BF16><<<attn_b8_grid(sm_count), AB_THREADS, C::SMEM, stream>>>(a);
   return cudaGetLastError();
 }
 

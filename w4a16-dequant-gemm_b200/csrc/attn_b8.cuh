@@ -3,6 +3,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "w4b_common.cuh"
 #include "w4b_kernels.h"
 
@@ -70,6 +72,29 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnB8& a, int i) {
   s.q0 = a.q_offsets ? a.q_offsets[i] : i;
   s.nq = a.q_offsets ? min(max(a.q_offsets[i + 1] - s.q0, 0), a.max_q) : 1;
   return s;
+}
+
+// The split of T units over G CTAs: CTA c has units [T c / G, T (c + 1) / G), and unit u is CTA ((u + 1) G - 1) / T's.
+// (64-bit division is some hundred instructions, so 32-bit where it suffices, and only where a row is split.)
+__device__ __forceinline__ int unit_owner(long long u, long long T, long long G) {
+  const unsigned long long n = (unsigned long long)(u + 1) * (unsigned long long)G - 1;
+  return n < 0x100000000ULL ? (int)((unsigned)n / (unsigned)T) : (int)(n / (unsigned long long)T);
+}
+__device__ __forceinline__ long long range_begin(long long T, long long c, long long G) {
+  const unsigned long long n = (unsigned long long)T * (unsigned long long)c;
+  return n < 0x100000000ULL ? (long long)((unsigned)n / (unsigned)G) : (long long)(n / (unsigned long long)G);
+}
+
+// Opts a kernel into `bytes` of shared memory, once per device (the call costs as much as half a launch).
+template <auto kernel>
+cudaError_t opt_in_smem(int bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && done[dev].load(std::memory_order_acquire))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_release);
+  return e;
 }
 
 }  // namespace w4b

@@ -37,6 +37,10 @@ constexpr int AC_TILE = 64;            // positions per tile
 constexpr int AC_THREADS = 512;
 constexpr int AC_WARPS = AC_THREADS / 32;
 constexpr int AC_MIN_UNITS = 4;        // units per CTA below which no further split pays
+#ifndef ACROW
+#define ACROW 4
+#endif
+constexpr int AC_ROW_COST = ACROW;         // units a group counts for besides its tiles: its start, join and store take that long
 
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -134,7 +138,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 struct RowGroup {
   int rows;    // query rows in use
   int tiles;   // position tiles any row sees
-  int units;   // at least one: a group that sees nothing still writes its zeros
+  int units;   // AC_ROW_COST of no tiles, then at least one: a group that sees nothing still writes its zeros
   bool split;  // both warpgroups share the rows
 };
 __device__ __forceinline__ RowGroup row_group(const AttnB8& a, const SeqInfo& s, int gi) {
@@ -144,7 +148,7 @@ __device__ __forceinline__ RowGroup row_group(const AttnB8& a, const SeqInfo& s,
   t.split = t.rows <= AC_ROWS;
   const int end = a.causal ? min(s.len, max(0, s.len - s.nq + (first + t.rows - 1) / a.group + 1)) : s.len;
   t.tiles = max(1, (end + AC_TILE - 1) / AC_TILE);
-  t.units = t.split ? (t.tiles + 1) / 2 : t.tiles;
+  t.units = (t.split ? (t.tiles + 1) / 2 : t.tiles) + AC_ROW_COST;
   return t;
 }
 __device__ __forceinline__ int row_groups(const AttnB8& a, const SeqInfo& s) {
@@ -174,6 +178,21 @@ struct ChunkSmem {
   static constexpr int BYTES = BAR_OFF + 256 + 1024;   // + alignment
 };
 
+// 16 bytes, or zeros
+__device__ __forceinline__ uint4 load_if(const uint8_t* p, bool on) {
+  uint4 v;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.u32 p, %5, 0;\n"
+      "mov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
+      "@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+      "}\n"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+
 // where a CTA's range of units starts
 struct RangeStart {
   long long u_begin, u_end, total, ctas;
@@ -191,13 +210,20 @@ struct Walk {
   __device__ __forceinline__ explicit Walk(const AttnB8& a, const RangeStart& b)
       : left((int)(b.u_end - b.u_begin)), seq(b.seq), head(b.head), gi(b.gi), r0(b.r0), it(0), s(seq_info(a, b.seq)) {}
   __device__ __forceinline__ bool more(const AttnB8& a) {
-    if (left <= 0) return false;
-    while (row_groups(a, s) == 0) s = seq_info(a, ++seq);  // sequences of the other kernel
-    t = row_group(a, s, gi);
-    n_units = min(t.units - r0, left);
-    tile0 = t.split ? 2 * r0 : r0;
-    n_tiles = t.split ? min(2 * n_units, t.tiles - tile0) : n_units;
-    return true;
+    while (left > 0) {
+      while (row_groups(a, s) == 0) s = seq_info(a, ++seq);  // sequences of the other kernel
+      t = row_group(a, s, gi);
+      n_units = min(t.units - r0, left);
+      const int u0 = max(0, r0 - AC_ROW_COST), u1 = r0 + n_units - AC_ROW_COST;  // units that stand for tiles
+      if (u1 > 0) {
+        tile0 = t.split ? 2 * u0 : u0;
+        n_tiles = min(t.split ? 2 * (u1 - u0) : u1 - u0, t.tiles - tile0);
+        return true;
+      }
+      n_tiles = 0;
+      next(a);
+    }
+    return false;
   }
   __device__ __forceinline__ void next(const AttnB8& a) {
     left -= n_units;
@@ -242,7 +268,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
     const long long G = most < (long long)gridDim.x ? most : (long long)gridDim.x;
     const long long cta = blockIdx.x;
     if (cta >= G) return;
-    const long long ub = T * cta / G, ue = T * (cta + 1) / G;
+    const long long ub = range_begin(T, cta, G), ue = range_begin(T, cta + 1, G);
     if (ub >= before && ub < before + mine) {
       long long off = ub - before, hu = 0;
       int i = i0;
@@ -399,40 +425,39 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
       const uint32_t dst = blk * (AC_TILE * 128) + row0 * 128;  // (ROWS is a multiple of 8: the swizzle is every pass's)
       const uint32_t dst0 = dst + (((2 * (lane & 3)) ^ (row0 & 7)) << 4), dst1 = dst + (((2 * (lane & 3) + 1) ^ (row0 & 7)) << 4);
       const int* bt = a.bt + (long long)k.seq * a.bt_stride;
-      const size_t slab = (size_t)k.head * a.npages;
+      const size_t slab = (size_t)k.head * a.npages, base = slab * a.page * D + piece * 16;
+      const uint8_t *kb = a.q_k + base, *vb = a.q_v + base;
       // Two tiles' codes in registers: while one is converted the other is on its way.
       struct Raw {
         uint4 k[PASSES], v[PASSES];
         float sk, sv;  // of block ct of the tile (threads 0-3)
       } raw[2];
-      // Pages are looked up one tile ahead of the loads that need them, all at once: looked up where they are used,
-      // four dependent loads in a row made this the slowest role (1600 cycles a tile).
-      int pg[PASSES], pg_s = -1;
+      // Lane b < 4 of every warp looks up the row of block b of a tile, one tile ahead of the loads that need it.
+      // (Looked up where it is used, four dependent loads in a row made this the slowest role: 1600 cycles a tile.)
+      int pg = -1, in_page = 0;
       const bool scales = ct < 4;
-      auto page_at = [&](int pos) { return pos < s.len ? __ldg(bt + a.page_div.div(pos)) : -1; };
       auto pages = [&](int r) {
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) pg[i] = page_at(r * AC_TILE + i * ROWS + row0);
-        if (scales) pg_s = page_at(r * AC_TILE + 16 * ct);
+        const int pos = r * AC_TILE + 16 * (lane & 3), pi = a.page_div.div(pos);
+        pg = pos < s.len && lane < 4 ? __ldg(bt + pi) : -1;
+        in_page = pos - pi * a.page;
       };
       auto load = [&](Raw& w, int r) {
+        const bool there = (unsigned)pg < (unsigned)a.npages;
+        const int row = there ? pg * a.page + in_page : -1;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-          const int pos = r * AC_TILE + i * ROWS + row0;
-          const size_t at = ((slab + pg[i]) * a.page + (pos - a.page_div.div(pos) * a.page)) * D + piece * 16;
-          const bool on = (unsigned)pg[i] < (unsigned)a.npages;  // (-1 behind the end)
-          w.k[i] = on ? __ldg((const uint4*)(a.q_k + at)) : make_uint4(0, 0, 0, 0);
-          w.v[i] = on ? __ldg((const uint4*)(a.q_v + at)) : make_uint4(0, 0, 0, 0);
+          const int b = D == 128 ? i : 2 * i + (row0 >> 4);  // block of this pass's row
+          const int first = __shfl_sync(0xffffffffu, row, b);
+          const int in = row0 & 15;
+          const bool on = first >= 0 && r * AC_TILE + 16 * b + in < s.len;
+          const size_t at = (size_t)(on ? first + in : 0) * D;
+          w.k[i] = load_if(kb + at, on);
+          w.v[i] = load_if(vb + at, on);
         }
         if (scales) {
-          w.sk = 0.0f;
-          w.sv = -1.0f;
-          if ((unsigned)pg_s < (unsigned)a.npages) {
-            w.sk = __ldg(a.s_k + slab + pg_s);
-            w.sv = __ldg(a.s_v + slab + pg_s);
-          } else if (r * AC_TILE + 16 * ct < s.len) {
-            atomicExch(a.status, ST_KV_PAGE);
-          }
+          w.sk = there ? __ldg(a.s_k + slab + pg) : 0.0f;
+          w.sv = there ? __ldg(a.s_v + slab + pg) : -1.0f;
+          if (!there && r * AC_TILE + 16 * ct < s.len) atomicExch(a.status, ST_KV_PAGE);
         }
       };
       auto store = [&](const uint4& raw, uint32_t tile, int i) {
@@ -671,9 +696,10 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
         }
         const long long G = start.ctas, T = start.total;
         const int cta = (int)blockIdx.x;
-        const long long row_begin = start.u_end - k.left - k.r0, row_end = row_begin + t.units;
-        const int first_cta = (int)(((row_begin + 1) * G - 1) / T), last_cta = (int)((row_end * G - 1) / T);
-        const bool whole = first_cta == last_cta;
+        const bool whole = k.r0 <= AC_ROW_COST && k.r0 + k.n_units == t.units;
+        const long long row_begin = start.u_end - k.left - k.r0;
+        const int first_cta = whole ? cta : unit_owner(row_begin + AC_ROW_COST, T, G);
+        const int last_cta = whole ? cta : unit_owner(row_begin + t.units - 1, T, G);
         uint16_t* out = (uint16_t*)a.out + (long long)(s.q0 + tq) * a.out_stride + (size_t)hq * D;
         auto finish = [&](float ms, float ls) {
           if (a.lse) a.lse[(long long)(s.q0 + tq) * (a.H * a.group) + hq] = row_lse(ms, ls);
@@ -776,10 +802,9 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
 
 template <int D, bool BF16>
 cudaError_t launch(const AttnB8& a, int sm_count, cudaStream_t stream) {
-  auto* k = attn_b8_chunk_kernel<D, BF16>;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem<D>::BYTES);
+  const cudaError_t e = opt_in_smem<attn_b8_chunk_kernel<D, BF16>>(ChunkSmem<D>::BYTES);
   if (e != cudaSuccess) return e;
-  k<<<sm_count, AC_THREADS, ChunkSmem<D>::BYTES, stream>>>(a);
+  attn_b8_chunk_kernel<D, BF16><<<sm_count, AC_THREADS, ChunkSmem<D>::BYTES, stream>>>(a);
   return cudaGetLastError();
 }
 
