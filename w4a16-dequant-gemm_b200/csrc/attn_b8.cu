@@ -132,7 +132,10 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
   const long long before = block_exclusive(mine, sums, T);
   const long long G = T < (long long)gridDim.x ? T : (long long)gridDim.x;
   const long long cta = blockIdx.x;
-  if (cta >= G) return;
+  if (cta >= G) {
+    if (cta == 0 && a.after_chunk) pdl_wait();
+    return;
+  }
   const long long u_begin = range_begin(T, cta, G), u_end = range_begin(T, cta + 1, G);
   if (u_begin >= before && u_begin < before + mine) {
     long long off = u_begin - before;
@@ -518,6 +521,8 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     u += step;
     off += step;
   }
+  // The chunk kernel before this one ran beside it; the stream's next kernel has to find both done.
+  if (cta == 0 && a.after_chunk) pdl_wait();
 }
 
 int attn_b8_grid(int sm_count) { return AB_CTAS_PER_SM * sm_count; }
@@ -527,8 +532,17 @@ cudaError_t launch(const AttnB8& a, int sm_count, cudaStream_t stream) {
   using C = AttnB8Kernel<D, NT, BF16>;
   const cudaError_t e = opt_in_smem<attn_b8_kernel<D, NT, BF16>>(C::SMEM);
   if (e != cudaSuccess) return e;
-  attn_b8_kernel<D, NT, BF16><<<attn_b8_grid(sm_count), AB_THREADS, C::SMEM, stream>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)attn_b8_grid(sm_count));
+  cfg.blockDim = dim3(AB_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.after_chunk ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, attn_b8_kernel<D, NT, BF16>, a);
 }
 
 }  // namespace
@@ -538,7 +552,8 @@ size_t attn_b8_ws_bytes(int sm_count) {
   return counter_bytes(grid) + (size_t)2 * grid * AB_MAX_COLS * (AB_MAX_D + 2) * sizeof(float);
 }
 
-cudaError_t attn_b8_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaStream_t stream, int* launches) {
+cudaError_t attn_b8_launch(const AttnB8& args, int D, int bf16, int sm_count, cudaStream_t stream, int* launches) {
+  AttnB8 a = args;
   const long long rows = (long long)a.max_q * a.group;
   const bool wide = rows > 8;
   *launches = 1;
@@ -547,6 +562,7 @@ cudaError_t attn_b8_launch(const AttnB8& a, int D, int bf16, int sm_count, cudaS
     // one sequence, or no row count below the threshold: nothing is left for the kernel below
     if (e != cudaSuccess || a.nseq == 1) return e;
     *launches = 2;
+    a.after_chunk = 1;
   }
 #define W4B_GO(DD)                                                                                      \
   (bf16 ? (wide ? launch<DD, 2, true>(a, sm_count, stream) : launch<DD, 1, true>(a, sm_count, stream)) \

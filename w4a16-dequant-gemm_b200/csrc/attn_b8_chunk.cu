@@ -37,10 +37,7 @@ constexpr int AC_TILE = 64;            // positions per tile
 constexpr int AC_THREADS = 512;
 constexpr int AC_WARPS = AC_THREADS / 32;
 constexpr int AC_MIN_UNITS = 4;        // units per CTA below which no further split pays
-#ifndef ACROW
-#define ACROW 4
-#endif
-constexpr int AC_ROW_COST = ACROW;         // units a group counts for besides its tiles: its start, join and store take that long
+constexpr int AC_ROW_COST = 4;         // units a group counts for besides its tiles: its start, join and store take that long
 
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -251,6 +248,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
   const uint32_t sm = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smp = smem_raw + (sm - smem_u32(smem_raw));
 
+  pdl_launch_dependents();  // the kernel for the short sequences may fill what this one leaves
   // ---- this CTA's range of units: warps take consecutive runs of sequences -------------------------------------
   {
     const int per = (a.nseq + AC_WARPS - 1) / AC_WARPS;
@@ -575,10 +573,16 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
       // While a row has seen nothing (`bare`) its reference point is 0; the first tile with a score sets it.
       float m = 0.0f, l = 0.0f;
       bool bare = true;
-      for (int j = j_first; j < n_tiles; j += j_step, ++mine) {
-        ok = ok && mbar_wait(s_full(w), (uint32_t)mine & 1u, a.status, ST_FLASH_TIMEOUT);
-        ok = __all_sync(0xffffffffu, ok);
+      // A barrier that is through costs some 150 cycles to ask all the same; so it is asked while the exponentials
+      // run, and waited for only if it was not through then. (Nothing the warp does depends on `ok` but its waits.)
+      auto await = [&](uint32_t bar, int phase, bool through) {
+        if (!through) ok = ok && mbar_wait(bar, (uint32_t)phase & 1u, a.status, ST_FLASH_TIMEOUT);
+        __syncwarp();
         tc_after_sync();
+      };
+      bool s_there = false;
+      for (int j = j_first; j < n_tiles; j += j_step, ++mine) {
+        await(s_full(w), mine, s_there);
         union {
           uint32_t u[AC_TILE];
           float f[AC_TILE];
@@ -610,11 +614,6 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
         }
 #pragma unroll
         for (int i = 0; i < AC_TILE; i += 2) top = max3(top, x.f[i], x.f[i + 1]);
-        if (j > j_first) {  // O and the place of the weights are free again
-          ok = ok && mbar_wait(o_done(w), (uint32_t)(mine - 1) & 1u, a.status, ST_FLASH_TIMEOUT);
-          ok = __all_sync(0xffffffffu, ok);
-          tc_after_sync();
-        }
         const bool move = bare ? top > -INFINITY : top > AB_SLACK;
         if (__any_sync(0xffffffffu, move)) {
           const float by = move ? top : 0.0f, f = bare ? 0.0f : ex2(-by);  // (nothing to scale while bare)
@@ -625,6 +624,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
 #pragma unroll
           for (int i = 0; i < AC_TILE / 2; ++i) x.p[i] = add2(x.p[i], neg);
           if (j > j_first) {
+            await(o_done(w), mine - 1, false);
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
@@ -637,18 +637,23 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
             tmem_wait_st();
           }
         }
+        // O and the place of the weights are free again; the next scores are there
+        // (unconditionally: a branch on the answer would wait for it here)
+        const bool o_test = mbar_test(o_done(w), (uint32_t)(mine - 1) & 1u), s_test = mbar_test(s_full(w), (uint32_t)(mine + 1) & 1u);
         uint32_t wt[32];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           f32x2 sum = pair(0.0f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float w0 = ex2(x.f[16 * b + 2 * i]), w1 = ex2(x.f[16 * b + 2 * i + 1]);
-            sum = add2(sum, pair(w0, w1));
-            wt[8 * b + i] = h2_as_u32(__floats2half2_rn(w0, w1));
+            const f32x2 e = pair(ex2(x.f[16 * b + 2 * i]), ex2(x.f[16 * b + 2 * i + 1]));
+            sum = add2(sum, e);
+            wt[8 * b + i] = h2_as_u32(__floats2half2_rn(lo(e), hi(e)));
           }
           l = fmaf(lo(sum) + hi(sum), inv[b], l);
         }
+        await(o_done(w), mine - 1, o_test || j == j_first);
+        s_there = s_test;
         tmem_st32(t_w + lane_off, wt);
         tmem_wait_st();
         signal(w_full(w));
@@ -658,11 +663,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
       if (t.split) asm volatile("bar.sync 3, 256;" ::: "memory");
       // ---- the row's result, or its part of it ----
       const bool some = j_first < n_tiles;  // (the second warpgroup of a shared group of one tile has none)
-      if (some) {
-        ok = ok && mbar_wait(o_done(w), (uint32_t)(mine - 1) & 1u, a.status, ST_FLASH_TIMEOUT);
-        ok = __all_sync(0xffffffffu, ok);
-        tc_after_sync();
-      }
+      if (some) await(o_done(w), mine - 1, false);
       float* join = (float*)(smp + L::JOIN_OFF);  // [row][2], then [D / 4][row][4]
       if (t.split && w == 1) {
         *(float2*)(join + 2 * rt) = make_float2(m, l);

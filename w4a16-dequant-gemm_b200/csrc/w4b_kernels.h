@@ -118,6 +118,7 @@ struct AttnB8 {
   void* ws;              // arrival counters (zero between launches), then partial results
   void* chunk_ws;        // the same for the chunk kernel
   int chunk_rows;        // sequences with at least this many query rows per key/value head are the chunk kernel's
+  int after_chunk;       // launched beside the chunk kernel (programmatic dependent launch): wait for it at the end
   int* status;
 };
 constexpr int kChunkRows = 48;
