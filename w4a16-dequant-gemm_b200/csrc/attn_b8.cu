@@ -459,17 +459,17 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
       }
     }
     if (!whole) {
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
+        __threadfence();  // (after the barrier: covers the whole CTA's writes, and below its reads)
         const int want = last_cta - first_cta + 1;
         const int got = atomicAdd(counters + first_cta, 1) + 1;
+        __threadfence();
         is_last = got == want;
         if (got == want) counters[first_cta] = 0;  // as the next launch expects it
       }
       __syncthreads();
       if (is_last) {
-        __threadfence();
         for (int e = tid; e < NC * LANES; e += AB_THREADS) {
           const int n = e / LANES, d = (e - n * LANES) * 8;
           if (n >= rows) continue;

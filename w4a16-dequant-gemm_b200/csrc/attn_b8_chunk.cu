@@ -194,6 +194,7 @@ __device__ __forceinline__ uint4 load_if(const uint8_t* p, bool on) {
 struct RangeStart {
   long long u_begin, u_end, total, ctas;
   int seq, head, gi, r0;
+  SeqInfo s;
 };
 
 // A role's walk over its CTA's row groups.
@@ -204,8 +205,8 @@ struct Walk {
   SeqInfo s;
   RowGroup t;
   int n_units, tile0, n_tiles;  // of the present group
-  __device__ __forceinline__ explicit Walk(const AttnB8& a, const RangeStart& b)
-      : left((int)(b.u_end - b.u_begin)), seq(b.seq), head(b.head), gi(b.gi), r0(b.r0), it(0), s(seq_info(a, b.seq)) {}
+  __device__ __forceinline__ explicit Walk(const RangeStart& b)
+      : left((int)(b.u_end - b.u_begin)), seq(b.seq), head(b.head), gi(b.gi), r0(b.r0), it(0), s(b.s) {}
   __device__ __forceinline__ bool more(const AttnB8& a) {
     while (left > 0) {
       while (row_groups(a, s) == 0) s = seq_info(a, ++seq);  // sequences of the other kernel
@@ -249,24 +250,62 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
   uint8_t* smp = smem_raw + (sm - smem_u32(smem_raw));
 
   pdl_launch_dependents();  // the kernel for the short sequences may fill what this one leaves
-  // ---- this CTA's range of units: warps take consecutive runs of sequences -------------------------------------
-  {
-    const int per = (a.nseq + AC_WARPS - 1) / AC_WARPS;
-    const int i0 = min(wid * per, a.nseq), i1 = min(i0 + per, a.nseq);
-    long long mine = 0;
-    for (int i = i0; i < i1; ++i) mine += a.H * head_units(a, seq_info(a, i), lane);
-    if (lane == 0) wsum[wid] = mine;
-    __syncthreads();
-    long long before = 0, T = 0;
-    for (int w = 0; w < AC_WARPS; ++w) {
-      if (w < wid) before += wsum[w];
-      T += wsum[w];
+  // ---- barriers and tensor memory by the last warp, beside the range by the others ------------------------------
+  const uint32_t bars = sm + L::BAR_OFF;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_free = [&](int s) { return bars + 32u + 8u * s; };
+  auto v_full = [&](int s) { return bars + 64u + 8u * s; };
+  auto v_free = [&](int s) { return bars + 96u + 8u * s; };
+  auto s_full = [&](int w) { return bars + 128u + 8u * w; };   // scores are there
+  auto s_free = [&](int w) { return bars + 144u + 8u * w; };   // scores have been read
+  auto w_full = [&](int w) { return bars + 160u + 8u * w; };   // weights are there
+  auto o_done = [&](int w) { return bars + 176u + 8u * w; };   // their product is done: O may be read, w overwritten
+  auto q_full = [&](int w) { return bars + 192u + 8u * w; };   // query rows are there
+  constexpr uint32_t COLS = 512;
+  if (wid == AC_WARPS - 1) {
+    if (lane == 0) {
+      for (int s = 0; s < L::STAGES; ++s) {
+        mbar_init(k_full(s), 4);  // the conversion warps
+        mbar_init(k_free(s), 1);
+        mbar_init(v_full(s), 4);
+        mbar_init(v_free(s), 1);
+      }
+      for (int w = 0; w < 2; ++w) {
+        mbar_init(s_full(w), 2);  // the MMAs' completion and the issuing thread itself (for the tile's factors)
+        mbar_init(s_free(w), 4);
+        mbar_init(w_full(w), 4);
+        mbar_init(o_done(w), 1);
+        mbar_init(q_full(w), 4);
+      }
+      mbar_init_fence();
     }
-    const long long most = (T + AC_MIN_UNITS - 1) / AC_MIN_UNITS;
-    const long long G = most < (long long)gridDim.x ? most : (long long)gridDim.x;
-    const long long cta = blockIdx.x;
-    if (cta >= G) return;
-    const long long ub = range_begin(T, cta, G), ue = range_begin(T, cta + 1, G);
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // This CTA's range of units: the other warps take consecutive runs of sequences.
+  constexpr int PLANNERS = AC_WARPS - 1;
+  const int per = (a.nseq + PLANNERS - 1) / PLANNERS;
+  const int i0 = min(wid * per, a.nseq), i1 = wid < PLANNERS ? min(i0 + per, a.nseq) : i0;
+  long long mine = 0;
+  for (int i = i0; i < i1; ++i) mine += a.H * head_units(a, seq_info(a, i), lane);
+  if (lane == 0) wsum[wid] = mine;
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  long long upto = lane < AC_WARPS ? wsum[lane] : 0;  // inclusive sums over the warps, by lane
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  const long long T = __shfl_sync(0xffffffffu, upto, 31), before = __shfl_sync(0xffffffffu, upto, wid) - mine;
+  const long long most = (T + AC_MIN_UNITS - 1) / AC_MIN_UNITS;
+  const long long G = most < (long long)gridDim.x ? most : (long long)gridDim.x;
+  const bool idle = (long long)blockIdx.x >= G;
+  if (!idle) {
+    const long long ub = range_begin(T, blockIdx.x, G), ue = range_begin(T, blockIdx.x + 1, G);
     if (ub >= before && ub < before + mine) {
       long long off = ub - before, hu = 0;
       int i = i0;
@@ -277,7 +316,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
         if (off < hu * a.H) break;
         off -= hu * a.H;
       }
-      const int head = (int)(off / hu);
+      const int head = (off | hu) < 0x7FFFFFFF ? (int)off / (int)hu : (int)(off / hu);
       off -= (long long)head * hu;
       int gi = 0;
       for (;; gi += 32) {  // 32 groups at a time
@@ -297,46 +336,12 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
         }
         off -= __shfl_sync(0xffffffffu, x, 31);
       }
-      if (lane == 0) start = RangeStart{ub, ue, T, G, i, head, gi, (int)off};
+      if (lane == 0) start = RangeStart{ub, ue, T, G, i, head, gi, (int)off, s};
     }
+  } else if (tid == 0) {
+    start.u_begin = start.u_end = 0;  // nothing to do: every role's walk is empty
   }
-
-  // ---- barriers, tensor memory ---------------------------------------------------------------------------------
-  const uint32_t bars = sm + L::BAR_OFF;
-  auto k_full = [&](int s) { return bars + 8u * s; };
-  auto k_free = [&](int s) { return bars + 32u + 8u * s; };
-  auto v_full = [&](int s) { return bars + 64u + 8u * s; };
-  auto v_free = [&](int s) { return bars + 96u + 8u * s; };
-  auto s_full = [&](int w) { return bars + 128u + 8u * w; };   // scores are there
-  auto s_free = [&](int w) { return bars + 144u + 8u * w; };   // scores have been read
-  auto w_full = [&](int w) { return bars + 160u + 8u * w; };   // weights are there
-  auto o_done = [&](int w) { return bars + 176u + 8u * w; };   // their product is done: O may be read, w overwritten
-  auto q_full = [&](int w) { return bars + 192u + 8u * w; };   // query rows are there
-  if (tid == 0) {
-    for (int s = 0; s < L::STAGES; ++s) {
-      mbar_init(k_full(s), 4);  // the conversion warps
-      mbar_init(k_free(s), 1);
-      mbar_init(v_full(s), 4);
-      mbar_init(v_free(s), 1);
-    }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(s_full(w), 2);  // the MMAs' completion and the issuing thread itself (for the tile's factors)
-      mbar_init(s_free(w), 4);
-      mbar_init(w_full(w), 4);
-      mbar_init(o_done(w), 1);
-      mbar_init(q_full(w), 4);
-    }
-    mbar_init_fence();
-  }
-  constexpr uint32_t COLS = 512;
-  if (wid == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tc_before_sync();
   __syncthreads();
-  tc_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
   // A wait that gave up: from there on this thread only walks through, so that every barrier of the warpgroups is met
@@ -348,7 +353,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
     // ------------------------------ MMA issue ------------------------------
     if (wid == 12 && elect_one()) {
       int mine = 0, other = 0, segments = 0;  // tiles of the warpgroups, row groups so far: phases
-      for (Walk k(a, start); k.more(a); k.next(a)) {
+      for (Walk k(start); k.more(a); k.next(a)) {
         const RowGroup& t = k.t;
         const int n_tiles = k.n_tiles, it = k.it;
         // D = F32, A = B = F16; S: B (K) K-major; O: B (V) MN-major
@@ -411,7 +416,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
   } else if (wid >= 8) {
     // ------------------------------ conversion ------------------------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    for (Walk k(a, start); k.more(a); k.next(a)) {
+    for (Walk k(start); k.more(a); k.next(a)) {
       const SeqInfo& s = k.s;
       const int n_tiles = k.n_tiles, tile0 = k.tile0, it = k.it;
       // A pass covers 128 pieces of 16 bytes: 16 rows (D = 128) or 32 (D = 64). Eight consecutive lanes take four
@@ -513,7 +518,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
     // ------------------------------ softmax: one thread per query row ------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     int mine = 0;  // tiles of this warpgroup so far: phase of its barriers
-    for (Walk k(a, start); k.more(a); k.next(a)) {
+    for (Walk k(start); k.more(a); k.next(a)) {
       const SeqInfo& s = k.s;
       const RowGroup& t = k.t;
       const int n_tiles = k.n_tiles, tile0 = k.tile0, it = k.it;
@@ -533,39 +538,55 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
       };
-      // Q to tensor memory as FP16 (BF16: by a power of two of the row's own, see attn_b8.cu)
+      // Q: each warp reads its 32 rows along the rows (one thread a row would touch 32 lines at every load: 6000
+      // cycles) into swizzled 128-byte rows of shared memory; then each thread makes its own row FP16 (BF16: by a
+      // power of two of the row's own, see attn_b8.cu), the first 64 dims to tensor memory, the others in place.
       float scale_row = 1.0f;
       {
-        const uint4* q = (const uint4*)((const uint16_t*)a.q + (long long)(s.q0 + tq) * a.q_stride + (size_t)hq * D);
+        constexpr int LPR = D / 8, RPL = 32 / LPR;  // lanes per row, rows per load
+        const uint32_t q_hi = sm + L::Q_OFF + w * (AC_ROWS * 128), q_lo = q_hi + (D == 128 ? 2 * AC_ROWS * 128 : 0);
+        const int piece = lane % LPR;
+        uint4 v[32 / RPL];
+#pragma unroll
+        for (int i = 0; i < 32 / RPL; ++i) {
+          const int r_in = (wid & 3) * 32 + i * RPL + lane / LPR + (t.split ? 0 : AC_ROWS * w);
+          const int r = k.gi * AC_GROUP + r_in, tok = r / a.group, hh = k.head * a.group + (r - tok * a.group);
+          v[i] = r_in < t.rows ? __ldg((const uint4*)((const uint16_t*)a.q + (long long)(s.q0 + tok) * a.q_stride + (size_t)hh * D) + piece)
+                               : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 32 / RPL; ++i) {
+          const int r = (wid & 3) * 32 + i * RPL + lane / LPR;
+          sts128((piece >= 8 ? q_hi : q_lo) + r * 128 + (((piece & 7) ^ (r & 7)) << 4), v[i]);
+        }
+        __syncwarp();
+        auto at = [&](int p) { return (p >= 8 ? q_hi : q_lo) + rt * 128 + (((p & 7) ^ (rt & 7)) << 4); };
         float up = 1.0f;
         if (BF16) {
           uint32_t top = 0;
-          for (int i = 0; i < D / 8; ++i) {
-            const uint4 v = on ? q[i] : make_uint4(0, 0, 0, 0);
-            top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
-                                         __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+#pragma unroll
+          for (int p = 0; p < LPR; ++p) {
+            const uint4 x = lds128(at(p));
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu),
+                                         __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
           }
           bf16_row_scale(max(top & 0xFFFFu, top >> 16), up, scale_row);
-        }
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t h[32];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint4 v = on ? q[8 * c + i] : make_uint4(0, 0, 0, 0);
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[4 * i + k] = BF16 ? bf16x2_to_h2(x[k], up) : x[k];
-          }
-          if (c == 0) {
-            tmem_st32(t_q + lane_off, h);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              sts128(sm + L::Q_OFF + w * (AC_ROWS * 128) + rt * 128 + ((i ^ (rt & 7)) << 4),
-                     make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]));
+          for (int p = 8; p < LPR; ++p) {
+            const uint4 x = lds128(at(p));
+            sts128(at(p), make_uint4(bf16x2_to_h2(x.x, up), bf16x2_to_h2(x.y, up), bf16x2_to_h2(x.z, up), bf16x2_to_h2(x.w, up)));
           }
         }
+        uint32_t h[32];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const uint4 x = lds128(at(p));
+          h[4 * p] = BF16 ? bf16x2_to_h2(x.x, up) : x.x;
+          h[4 * p + 1] = BF16 ? bf16x2_to_h2(x.y, up) : x.y;
+          h[4 * p + 2] = BF16 ? bf16x2_to_h2(x.z, up) : x.z;
+          h[4 * p + 3] = BF16 ? bf16x2_to_h2(x.w, up) : x.w;
+        }
+        tmem_st32(t_q + lane_off, h);
         if (D == 128) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tmem_wait_st();
         signal(q_full(w));
@@ -715,12 +736,12 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
           }
         };
         int* counter = (int*)a.chunk_ws + 2 * first_cta + w;
+        const int want = last_cta - first_cta + 1;
         constexpr size_t PART = (size_t)AC_ROWS * (D + 2);  // floats per warpgroup
         float* parts = (float*)((uint8_t*)a.chunk_ws + counter_bytes(2 * (int)gridDim.x)) + w * PART;
         auto slot = [&](int k) { return parts + (size_t)(k == first_cta ? 2 * k + 1 : 2 * k) * (2 * PART); };
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
+        // this CTA's 32 columns of chunk c
+        auto own = [&](int c, float* o) {
           tmem_ld32(t_o + 32 * c + lane_off, (uint32_t*)o);
           tmem_wait_ld();
           if (t.split) {
@@ -734,37 +755,65 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
               o[4 * i + 3] = fmaf(o[4 * i + 3], f0, v.w * f1);
             }
           }
-          if (whole) {
-            if (on) store32(c, o, row_norm(l));
-          } else {
-            // [D / 4][row][4]: consecutive rows next to each other
-            float* p = slot(cta) + 2 * AC_ROWS + (size_t)(8 * c * AC_ROWS + rt) * 4;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *(float4*)(p + (size_t)i * AC_ROWS * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-        }
-        tc_before_sync();
+        };
         if (whole) {
+          const float norm = row_norm(l);
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            own(c, o);
+            if (on) store32(c, o, norm);
+          }
           if (on) finish(m, l);
         } else {
-          *(float2*)(slot(cta) + 2 * rt) = make_float2(m, l);
-          __threadfence();
-          asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
-          if (rt == 0) {
-            const int want = last_cta - first_cta + 1;
-            const bool last = atomicAdd(counter, 1) + 1 == want;
-            is_last[w] = last;
-            if (last) *counter = 0;  // as the next launch expects it
+          // The CTA that comes last joins all parts, in CTA order, its own from tensor memory. One that finds itself
+          // last already need not write its part.
+          auto ask = [&](bool add) {
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
+            if (rt == 0) {
+              int before;
+              if (add) {
+                // release (after the barrier: the whole warpgroup's writes) and acquire
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+              } else {
+                asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(before) : "l"(counter) : "memory");
+              }
+              is_last[w] = before == want - 1;
+              if (before == want - 1) *counter = 0;  // as the next launch expects it
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
+            return is_last[w] != 0;
+          };
+          bool last = ask(false);
+          if (!last) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              own(c, o);
+              // [D / 4][row][4]: consecutive rows next to each other
+              float* p = slot(cta) + 2 * AC_ROWS + (size_t)(8 * c * AC_ROWS + rt) * 4;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                *(float4*)(p + (size_t)i * AC_ROWS * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+            *(float2*)(slot(cta) + 2 * rt) = make_float2(m, l);
+            last = ask(true);
           }
-          asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
-          if (is_last[w] && on) {
-            __threadfence();
+          if (last) {
+            auto ml = [&](int k) { return k == cta ? make_float2(m, l) : __ldcg((const float2*)(slot(k) + 2 * rt)); };
             float ms = AB_NONE, ls = 0.0f;
-            for (int k = first_cta; k <= last_cta; ++k) ms = fmaxf(ms, __ldcg(slot(k) + 2 * rt));
-            for (int k = first_cta; k <= last_cta; ++k) {
-              const float2 ml = __ldcg((const float2*)(slot(k) + 2 * rt));
-              ls = fmaf(ml.y, ex2(ml.x - ms), ls);
+            for (int k0 = first_cta; k0 <= last_cta; k0 += 4) {
+              float2 v[4];
+#pragma unroll
+              for (int b = 0; b < 4; ++b) v[b] = ml(min(k0 + b, last_cta));
+              float mn = ms;
+#pragma unroll
+              for (int b = 0; b < 4; ++b) mn = fmaxf(mn, v[b].x);
+              ls *= ex2(ms - mn);
+              ms = mn;
+#pragma unroll
+              for (int b = 0; b < 4; ++b)
+                if (k0 + b <= last_cta) ls = fmaf(v[b].y, ex2(v[b].x - ms), ls);
             }
             const float norm = row_norm(ls);
 #pragma unroll 1
@@ -774,31 +823,31 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
               for (int i = 0; i < 32; ++i) v[i] = 0.0f;
 #pragma unroll 1
               for (int k = first_cta; k <= last_cta; ++k) {
-                const float* p = slot(k) + 2 * AC_ROWS + (size_t)(8 * c * AC_ROWS + rt) * 4;
-                const float f = ex2(__ldcg(slot(k) + 2 * rt) - ms);
-                float4 o[8];
+                const float f = ex2(ml(k).x - ms);
+                float o[32];
+                if (k == cta) {
+                  own(c, o);
+                } else {
+                  const float* p = slot(k) + 2 * AC_ROWS + (size_t)(8 * c * AC_ROWS + rt) * 4;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = __ldcg((const float4*)(p + (size_t)i * AC_ROWS * 4));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  v[4 * i] = fmaf(o[i].x, f, v[4 * i]);
-                  v[4 * i + 1] = fmaf(o[i].y, f, v[4 * i + 1]);
-                  v[4 * i + 2] = fmaf(o[i].z, f, v[4 * i + 2]);
-                  v[4 * i + 3] = fmaf(o[i].w, f, v[4 * i + 3]);
+                  for (int i = 0; i < 8; ++i) *(float4*)(o + 4 * i) = __ldcg((const float4*)(p + (size_t)i * AC_ROWS * 4));
                 }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = fmaf(o[i], f, v[i]);
               }
-              store32(c, v, norm);
+              if (on) store32(c, v, norm);
             }
-            finish(ms, ls);
+            if (on) finish(ms, ls);
           }
         }
+        tc_before_sync();
       }
       if (t.split) asm volatile("bar.sync 3, 256;" ::: "memory");  // the join buffer is free again
     }
   }
   tc_before_sync();
   __syncthreads();
-  if (wid == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
+  if (wid == AC_WARPS - 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
 }
 
 template <int D, bool BF16>
