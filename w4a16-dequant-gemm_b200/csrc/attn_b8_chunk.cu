@@ -37,7 +37,7 @@ constexpr int AC_TILE = 64;            // positions per tile
 constexpr int AC_THREADS = 512;
 constexpr int AC_WARPS = AC_THREADS / 32;
 constexpr int AC_MIN_UNITS = 4;        // units per CTA below which no further split pays
-constexpr int AC_ROW_COST = 4;         // units a group counts for besides its tiles: its start, join and store take that long
+constexpr int AC_ROW_COST = 6;         // units a group counts for besides its tiles: its start, join and store take that long
 
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
