@@ -462,6 +462,27 @@ def test_attention_several_tokens(case, dtype, causal):
     assert w4.device_status() == 0
 
 
+@pytest.mark.parametrize("many", [1, 17], ids=["single", "rows"])
+def test_attention_thousands_of_sequences(many):
+    """5200 short sequences: every work range covers dozens, some of them without tokens or positions."""
+    n = 5200
+    rng = np.random.default_rng(7)
+    nq = (rng.integers(0, 8, n) > 0).astype(int) * many
+    p = Problem(rng.integers(0, 30, n).tolist(), nq.tolist(), 1, 2, 64, 16, F16, False, seed=30)
+    p.check(*p.run())
+    assert w4.device_status() == 0
+
+
+def test_attention_mixed_batch():
+    """Single tokens, drafts and prompt chunks side by side: both kernels in one call, sequences of one between the other's."""
+    rng = np.random.default_rng(8)
+    nq = [int(x) for x in rng.choice([1, 1, 1, 2, 5, 60, 300], 70)]
+    lens = [int(x) + q for x, q in zip(rng.integers(0, 700, 70), nq)]
+    p = Problem(lens, nq, 2, 4, 128, 32, BF16, True, seed=31)
+    p.check(*p.run())
+    assert w4.device_status() == 0
+
+
 @pytest.mark.parametrize("nq", [1, 3, 70])
 def test_attention_scales_far_apart(nq):
     """Pages whose scales differ by 2^50: the large ones decide the values, all decide the weights."""

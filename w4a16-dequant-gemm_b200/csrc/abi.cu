@@ -57,7 +57,9 @@ struct Scratch {
     cudaError_t e = cudaMalloc(&nb, want);
     if (e != cudaSuccess) return e;
     if (zero) {
+      // (waited for: the caller's stream need not be ordered behind the default stream, where this runs)
       e = cudaMemset(nb, 0, want);
+      if (e == cudaSuccess) e = cudaStreamSynchronize(0);
       if (e != cudaSuccess) {
         cudaFree(nb);
         return e;

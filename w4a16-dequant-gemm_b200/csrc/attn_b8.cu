@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
   const int i_begin = min(tid * per, a.nseq), i_end = min(i_begin + per, a.nseq);
   long long mine = 0;
   int tiles, units;
+#pragma unroll 4
   for (int i = i_begin; i < i_end; ++i) mine += seq_units<NC>(a, seq_info(a, i), tiles, units);
   long long T;
   const long long before = block_exclusive(mine, sums, T);

@@ -36,6 +36,7 @@ constexpr int AC_GROUP = 2 * AC_ROWS;  // per CTA
 constexpr int AC_TILE = 64;            // positions per tile
 constexpr int AC_THREADS = 512;
 constexpr int AC_WARPS = AC_THREADS / 32;
+constexpr int AC_LIST = 32;            // sequences of a CTA's range that are looked up beforehand
 constexpr int AC_MIN_UNITS = 4;        // units per CTA below which no further split pays
 constexpr int AC_ROW_COST = 6;         // units a group counts for besides its tiles: its start, join and store take that long
 
@@ -152,14 +153,31 @@ __device__ __forceinline__ int row_groups(const AttnB8& a, const SeqInfo& s) {
   const int rows = s.nq * a.group;
   return rows >= a.chunk_rows ? (rows + AC_GROUP - 1) / AC_GROUP : 0;
 }
-// Units of one head of a sequence, by a warp (the same value in every lane).
-__device__ __forceinline__ long long head_units(const AttnB8& a, const SeqInfo& s, int lane) {
-  const int n = row_groups(a, s);
-  long long sum = 0;
-  for (int gi = lane; gi < n; gi += 32) sum += row_group(a, s, gi).units;
+// Units of sequences i0 + lane (lane < n <= 32), all heads: a sequence of many groups by the whole warp, 32 at a time.
+__device__ __forceinline__ long long warp_units(const AttnB8& a, int i0, int n, int lane) {
+  SeqInfo s = {0, 0, 0};
+  if (lane < n) s = seq_info(a, i0 + lane);
+  const int groups = row_groups(a, s);
+  int mine = 0;
+  if (groups <= 8)
+    for (int gi = 0; gi < groups; ++gi) mine += row_group(a, s, gi).units;
+  for (uint32_t big = __ballot_sync(0xffffffffu, groups > 8); big != 0; big &= big - 1) {
+    const int k = __ffs(big) - 1, all = __shfl_sync(0xffffffffu, groups, k);
+    const SeqInfo t = {__shfl_sync(0xffffffffu, s.len, k), 0, __shfl_sync(0xffffffffu, s.nq, k)};
+    int sum = 0;
+    for (int gi = lane; gi < all; gi += 32) sum += row_group(a, t, gi).units;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == k) mine = sum;
+  }
+  return (long long)a.H * mine;
+}
+__device__ __forceinline__ long long warp_scan(long long v, int lane) {  // inclusive
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  return sum;
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
 }
 
 template <int D>
@@ -193,23 +211,34 @@ __device__ __forceinline__ uint4 load_if(const uint8_t* p, bool on) {
 // where a CTA's range of units starts
 struct RangeStart {
   long long u_begin, u_end, total, ctas;
-  int seq, head, gi, r0;
-  SeqInfo s;
+  int head, gi, r0;
+  int count;               // sequences with work in the range (the first AC_LIST of them are listed)
+  int seq[AC_LIST];
+  SeqInfo s[AC_LIST];
 };
 
 // A role's walk over its CTA's row groups.
 struct Walk {
   int left;  // units still to do
+  int idx;   // the sequence's place in the list
   int seq, head, gi, r0;
   int it;    // tiles so far: stage and phase of the rings
   SeqInfo s;
   RowGroup t;
   int n_units, tile0, n_tiles;  // of the present group
   __device__ __forceinline__ explicit Walk(const RangeStart& b)
-      : left((int)(b.u_end - b.u_begin)), seq(b.seq), head(b.head), gi(b.gi), r0(b.r0), it(0), s(b.s) {}
-  __device__ __forceinline__ bool more(const AttnB8& a) {
+      : left((int)(b.u_end - b.u_begin)), idx(0), seq(b.seq[0]), head(b.head), gi(b.gi), r0(b.r0), it(0), s(b.s[0]) {}
+  __device__ __forceinline__ void next_sequence(const AttnB8& a, const RangeStart& b) {
+    if (++idx < b.count) {
+      seq = b.seq[idx];
+      s = b.s[idx];
+    } else {  // behind the list: one after the other, past those of the other kernel
+      do s = seq_info(a, ++seq);
+      while (row_groups(a, s) == 0);
+    }
+  }
+  __device__ __forceinline__ bool more(const AttnB8& a, const RangeStart& b) {
     while (left > 0) {
-      while (row_groups(a, s) == 0) s = seq_info(a, ++seq);  // sequences of the other kernel
       t = row_group(a, s, gi);
       n_units = min(t.units - r0, left);
       const int u0 = max(0, r0 - AC_ROW_COST), u1 = r0 + n_units - AC_ROW_COST;  // units that stand for tiles
@@ -219,11 +248,11 @@ struct Walk {
         return true;
       }
       n_tiles = 0;
-      next(a);
+      next(a, b);
     }
     return false;
   }
-  __device__ __forceinline__ void next(const AttnB8& a) {
+  __device__ __forceinline__ void next(const AttnB8& a, const RangeStart& b) {
     left -= n_units;
     it += n_tiles;
     r0 = 0;
@@ -231,7 +260,7 @@ struct Walk {
       gi = 0;
       if (++head == a.H) {
         head = 0;
-        if (left > 0) s = seq_info(a, ++seq);
+        if (left > 0) next_sequence(a, b);
       }
     }
   }
@@ -289,17 +318,13 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
   const int per = (a.nseq + PLANNERS - 1) / PLANNERS;
   const int i0 = min(wid * per, a.nseq), i1 = wid < PLANNERS ? min(i0 + per, a.nseq) : i0;
   long long mine = 0;
-  for (int i = i0; i < i1; ++i) mine += a.H * head_units(a, seq_info(a, i), lane);
+  for (int i = i0; i < i1; i += 32) mine += warp_units(a, i, min(32, i1 - i), lane);
+  mine = __shfl_sync(0xffffffffu, warp_scan(mine, lane), 31);
   if (lane == 0) wsum[wid] = mine;
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
-  long long upto = lane < AC_WARPS ? wsum[lane] : 0;  // inclusive sums over the warps, by lane
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += o;
-  }
+  const long long upto = warp_scan(lane < AC_WARPS ? wsum[lane] : 0, lane);  // over the warps
   const long long T = __shfl_sync(0xffffffffu, upto, 31), before = __shfl_sync(0xffffffffu, upto, wid) - mine;
   const long long most = (T + AC_MIN_UNITS - 1) / AC_MIN_UNITS;
   const long long G = most < (long long)gridDim.x ? most : (long long)gridDim.x;
@@ -307,36 +332,55 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
   if (!idle) {
     const long long ub = range_begin(T, blockIdx.x, G), ue = range_begin(T, blockIdx.x + 1, G);
     if (ub >= before && ub < before + mine) {
-      long long off = ub - before, hu = 0;
-      int i = i0;
-      SeqInfo s;
-      for (;; ++i) {
-        s = seq_info(a, i);
-        hu = head_units(a, s, lane);
-        if (off < hu * a.H) break;
-        off -= hu * a.H;
-      }
-      const int head = (off | hu) < 0x7FFFFFFF ? (int)off / (int)hu : (int)(off / hu);
-      off -= (long long)head * hu;
-      int gi = 0;
-      for (;; gi += 32) {  // 32 groups at a time
-        const int n = row_groups(a, s);
-        long long v = gi + lane < n ? row_group(a, s, gi + lane).units : 0, x = v;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const long long o = __shfl_up_sync(0xffffffffu, x, d);
-          if (lane >= d) x += o;
+      // the sequence that unit ub is in, and those after it up to unit ue
+      long long base = before;
+      int count = 0;
+      for (int i = i0; i < a.nseq && base < ue; i += 32) {
+        const int n = min(32, a.nseq - i);
+        const long long v = warp_units(a, i, n, lane), end = base + warp_scan(v, lane);
+        const bool in = v > 0 && end > ub && end - v < ue;
+        const uint32_t all = __ballot_sync(0xffffffffu, in);
+        const int at = count + __popc(all & ((1u << lane) - 1));
+        if (in && at < AC_LIST) {
+          start.seq[at] = i + lane;
+          start.s[at] = seq_info(a, i + lane);
         }
-        const uint32_t in = __ballot_sync(0xffffffffu, off < x);
-        if (in != 0) {
-          const int k = __ffs(in) - 1;
-          off -= __shfl_sync(0xffffffffu, x - v, k);
-          gi += k;
-          break;
+        if (count == 0 && all != 0) {
+          const int k = __ffs(all) - 1;
+          const long long first = __shfl_sync(0xffffffffu, end - v, k), units = __shfl_sync(0xffffffffu, v, k);
+          const SeqInfo s = seq_info(a, i + k);
+          long long off = ub - first;
+          const long long hu = (unsigned long long)units < 0x100000000ULL ? (unsigned)units / (unsigned)a.H : units / a.H;
+          const int head = (off | hu) < 0x7FFFFFFF ? (int)off / (int)hu : (int)(off / hu);
+          off -= (long long)head * hu;
+          int gi = 0;
+          for (;; gi += 32) {  // 32 groups at a time
+            const long long u = gi + lane < row_groups(a, s) ? row_group(a, s, gi + lane).units : 0, x = warp_scan(u, lane);
+            const uint32_t here = __ballot_sync(0xffffffffu, off < x);
+            if (here != 0) {
+              const int b = __ffs(here) - 1;
+              off -= __shfl_sync(0xffffffffu, x - u, b);
+              gi += b;
+              break;
+            }
+            off -= __shfl_sync(0xffffffffu, x, 31);
+          }
+          if (lane == 0) {
+            start.head = head;
+            start.gi = gi;
+            start.r0 = (int)off;
+          }
         }
-        off -= __shfl_sync(0xffffffffu, x, 31);
+        count += __popc(all);
+        base = __shfl_sync(0xffffffffu, end, 31);
       }
-      if (lane == 0) start = RangeStart{ub, ue, T, G, i, head, gi, (int)off, s};
+      if (lane == 0) {
+        start.u_begin = ub;
+        start.u_end = ue;
+        start.total = T;
+        start.ctas = G;
+        start.count = min(count, AC_LIST);
+      }
     }
   } else if (tid == 0) {
     start.u_begin = start.u_end = 0;  // nothing to do: every role's walk is empty
@@ -353,7 +397,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
     // ------------------------------ MMA issue ------------------------------
     if (wid == 12 && elect_one()) {
       int mine = 0, other = 0, segments = 0;  // tiles of the warpgroups, row groups so far: phases
-      for (Walk k(start); k.more(a); k.next(a)) {
+      for (Walk k(start); k.more(a, start); k.next(a, start)) {
         const RowGroup& t = k.t;
         const int n_tiles = k.n_tiles, it = k.it;
         // D = F32, A = B = F16; S: B (K) K-major; O: B (V) MN-major
@@ -416,7 +460,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
   } else if (wid >= 8) {
     // ------------------------------ conversion ------------------------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    for (Walk k(start); k.more(a); k.next(a)) {
+    for (Walk k(start); k.more(a, start); k.next(a, start)) {
       const SeqInfo& s = k.s;
       const int n_tiles = k.n_tiles, tile0 = k.tile0, it = k.it;
       // A pass covers 128 pieces of 16 bytes: 16 rows (D = 128) or 32 (D = 64). Eight consecutive lanes take four
@@ -518,7 +562,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
     // ------------------------------ softmax: one thread per query row ------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     int mine = 0;  // tiles of this warpgroup so far: phase of its barriers
-    for (Walk k(start); k.more(a); k.next(a)) {
+    for (Walk k(start); k.more(a, start); k.next(a, start)) {
       const SeqInfo& s = k.s;
       const RowGroup& t = k.t;
       const int n_tiles = k.n_tiles, tile0 = k.tile0, it = k.it;
