@@ -6,8 +6,8 @@
 //   w = 2^(X - m),  O^T[d][n] += sum_pos Vcode[pos][d] * w[pos][n],  l[n] += w / s_v
 // with m a reference point near the running maximum of X: taking log2(s_v) into the exponent puts V's scale into the
 // weights for free, whatever its size, and w / s_v is the plain softmax weight. out = O / l, lse = ln 2 (m + log2 l).
-// m moves only when some X exceeds it by more than 8 (a warp vote), so the usual block needs no reduction across
-// lanes: weights up to 2^8 are exact-enough halves, sums are FP32.
+// m moves only when some X exceeds it by more than 14 (a warp vote), so the usual block needs no reduction across
+// lanes: weights up to 2^14 are halves like others, and sums are FP32.
 //
 // Both products run on mma.sync.m16n8k16 with the CACHE as the 16-row operand and the query rows as the 8 columns
 // (a decode step has 1 to 16 rows: as the 128-row operand of the larger tensor instructions they would leave most of
@@ -24,6 +24,11 @@
 // Split: all work - 64-position units of all (sequence, head, column tile) rows in order - is cut into equal ranges,
 // one per CTA, whatever the lengths; the lengths are on the device, so every CTA sums them itself. A row that spans
 // CTAs is joined by whichever of them arrives last, in CTA order (bit-identical from run to run).
+//
+// Measured (device time in a graph): 4 sequences x 131,072 positions, 32 query heads on 8 of 128: 191 us = 5.6 TB/s,
+// 0.86 of the measured copy rate; 64 sequences of 100 to 8192 positions, 64 heads on 8 of 128: 55 us = 4.6 TB/s (0.69;
+// 5 us of it are launch, the sums over the lengths and the first loads, 70 us without AB_ROW_COST: CTAs with many
+// short rows came late); one sequence of 778: 8 us.
 #include "attn_b8.cuh"
 
 namespace w4b {
@@ -32,11 +37,12 @@ namespace {
 constexpr int AB_WARPS = 4;
 constexpr int AB_THREADS = 32 * AB_WARPS;
 constexpr int AB_CTAS_PER_SM = 4;
-constexpr int AB_STAGES = 3;
+constexpr int AB_STAGES = 3;     // 16 warps x 3 x 4 KB: all the shared memory there is
 constexpr int AB_UNIT = 64;      // positions per work unit: one block of 16 per warp
 constexpr int AB_ROW_COST = 2;   // units a row counts for besides its positions: its start, join and store take that long
 constexpr int AB_JOIN = 16;      // parts of a row up to which one CTA joins them all
 constexpr int AB_MAX_COLS = 16;  // query rows per column tile
+
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
