@@ -521,8 +521,10 @@ def test_attention_missing_pages(nq):
     p.check(out, lse, missing=[(0, 3), (0, 12), (1, 0), (1, 1), (1, 2), (1, 3)])
 
 
-def test_attention_nan_stays_in_its_rows():
-    p = Problem([100, 60], [2, 3], 2, 2, 64, 16, F16, True, seed=9)
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq", [[2, 3], [40, 90]], ids=["few", "many"])
+def test_attention_nan_stays_in_its_rows(nq, dtype):
+    p = Problem([200, 160], nq, 2, 2, 64, 16, dtype, True, seed=9)
     clean, clean_lse = p.run()
     q = p.q.clone()
     q[1, 2, 5], q[3, 0, 0] = math.nan, math.inf
