@@ -37,7 +37,6 @@ namespace {
 constexpr int AB_WARPS = 4;
 constexpr int AB_THREADS = 32 * AB_WARPS;
 constexpr int AB_CTAS_PER_SM = 4;
-constexpr int AB_STAGES = 3;     // 16 warps x 3 x 4 KB: all the shared memory there is
 constexpr int AB_UNIT = 64;      // positions per work unit: one block of 16 per warp
 constexpr int AB_ROW_COST = 2;   // units a row counts for besides its positions: its start, join and store take that long
 constexpr int AB_JOIN = 16;      // parts of a row up to which one CTA joins them all
@@ -46,6 +45,9 @@ constexpr int AB_MAX_COLS = 16;  // query rows per column tile
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -106,7 +108,8 @@ struct AttnB8Kernel {
   static constexpr int PIECES = D / 16;             // 16-byte pieces per row
   static constexpr int SIDE = 16 * D;               // bytes of K (or V) in a block
   static constexpr int STAGE = 2 * SIDE + 16;       // + s_k, s_v
-  static constexpr int RING = AB_STAGES * STAGE;    // per warp
+  static constexpr int STAGES = 384 / D;            // 16 warps x 3 x 4 KB (6 x 2 KB): all the shared memory there is
+  static constexpr int RING = STAGES * STAGE;       // per warp
   static constexpr int OPITCH = D + 8;              // floats per column of the merge buffer
   static constexpr int MERGE = AB_WARPS * NC * (OPITCH + 2) * 4;
   static constexpr int SMEM = (AB_WARPS * RING > MERGE ? AB_WARPS * RING : MERGE);
@@ -127,6 +130,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
   __shared__ long long sums[AB_WARPS];
   __shared__ long long found_off;
   __shared__ int found_seq, is_last;
+  __shared__ SeqInfo found_info;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
 
   // ---- this CTA's range of units -----------------------------------------------------------------------------
@@ -148,13 +152,16 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
   if (u_begin >= before && u_begin < before + mine) {
     long long off = u_begin - before;
     int i = i_begin;
+    SeqInfo s;
     for (;; ++i) {
-      const long long n = seq_units<NC>(a, seq_info(a, i), tiles, units);
+      s = seq_info(a, i);
+      const long long n = seq_units<NC>(a, s, tiles, units);
       if (off < n) break;
       off -= n;
     }
     found_seq = i;
     found_off = off;
+    found_info = s;
   }
   __syncthreads();
   int seq = found_seq;
@@ -165,11 +172,11 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
   float* parts = (float*)((uint8_t*)a.ws + counter_bytes(3 * (int)gridDim.x));
   const uint32_t ring = smem_u32(smem) + wid * C::RING;
 
+  SeqInfo s = found_info;
   while (u < u_end) {
-    const SeqInfo s = seq_info(a, seq);
     const long long seq_n = seq_units<NC>(a, s, tiles, units);
     if (off >= seq_n) {
-      ++seq;
+      s = seq_info(a, ++seq);
       off = 0;
       continue;
     }
@@ -197,21 +204,40 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     const int* bt = a.bt + (long long)seq * a.bt_stride;
     const size_t slab = (size_t)head * a.npages;
     auto position = [&](int j) { return p_begin + (wid + j * AB_WARPS) * 16; };
-    auto page_of = [&](int j) { return j < mine_n ? bt[a.page_div.div(position(j))] : 0; };
-    auto issue = [&](int j, int pg) {
-      const uint32_t st = ring + (j % AB_STAGES) * C::STAGE;
+    // the page of block j (-1 behind the end), and the row of the page it starts at
+    struct Place {
+      int pg, in;
+    };
+    auto page_of = [&](int j) {
+      const int p0 = position(j), pi = a.page_div.div(p0);
+      return Place{j < mine_n ? bt[pi] : -1, p0 - pi * a.page};
+    };
+    // where this lane's 16 bytes of a copy go: rows lane / PIECES, then on from there
+    const uint32_t lane0 = C::piece(lane / C::PIECES, lane % C::PIECES);
+    const uint32_t lane1 = D == 128 ? C::piece(lane / C::PIECES + 4, lane % C::PIECES) - 512 : lane0;
+    auto issue = [&](int j, Place at) {
+      const uint32_t st = ring + (j % C::STAGES) * C::STAGE;
       if (j < mine_n) {
-        const int p0 = position(j);
+        const int pg = at.pg;
         const bool good = (unsigned)pg < (unsigned)a.npages;
-        const size_t r = (slab + (good ? pg : 0)) * a.page + (p0 - a.page_div.div(p0) * a.page);
-        const uint8_t* ks = a.q_k + r * D;
-        const uint8_t* vs = a.q_v + r * D;
+        const size_t r = (slab + (good ? pg : 0)) * a.page + at.in;
+        const uint8_t* ks = a.q_k + r * D + lane * 16;
+        const uint8_t* vs = a.q_v + r * D + lane * 16;
+        if (good && position(j) + 16 <= s.len) {
 #pragma unroll
-        for (int i = 0; i < C::SIDE / 512; ++i) {
-          const int e = i * 32 + lane, rr = e / C::PIECES, jj = e - rr * C::PIECES;
-          const bool on = good && p0 + rr < s.len;
-          cp_async16_zfill(st + C::piece(rr, jj), ks + (on ? e * 16 : 0), on);
-          cp_async16_zfill(st + C::SIDE + C::piece(rr, jj), vs + (on ? e * 16 : 0), on);
+          for (int i = 0; i < C::SIDE / 512; ++i) {
+            const uint32_t to = st + ((i & 1) ? lane1 : lane0) + i * 512;
+            cp_async16(to, ks + i * 512);
+            cp_async16(to + C::SIDE, vs + i * 512);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < C::SIDE / 512; ++i) {
+            const uint32_t to = st + ((i & 1) ? lane1 : lane0) + i * 512;
+            const bool on = good && position(j) + (i * 32 + lane) / C::PIECES < s.len;
+            cp_async16_zfill(to, ks + (on ? i * 512 : 0), on);
+            cp_async16_zfill(to + C::SIDE, vs + (on ? i * 512 : 0), on);
+          }
         }
         if (lane < 2) {
           const float* sc = (lane == 0 ? a.s_k : a.s_v) + slab + (good ? pg : 0);
@@ -225,18 +251,12 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
       }
       cp_async_commit();
     };
-    int pg_next = page_of(0);
-#pragma unroll
-    for (int j = 0; j < AB_STAGES - 1; ++j) {
-      const int pg = pg_next;
-      pg_next = page_of(j + 1);
-      issue(j, pg);
-    }
-
     // ---- query rows as operand registers: lane (g, c) holds row g, dims 16 i + 4 c .. + 3 ----------------------
+    // (read between the first look-up of a page and the copies that wait for it)
     uint32_t qf[NT][C::KSTEPS][2];
     float fs[NT][2];     // per column (2c, 2c + 1): score factor without s_k
     int lim[NT][2];      // per column: positions it sees
+    Place pg_next = page_of(0);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int n = t * 8 + g, r = tile * NC + n;
@@ -244,33 +264,37 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
       const int tq = on ? r / a.group : 0, hh = on ? r - tq * a.group : 0;
       const uint16_t* qrow =
           (const uint16_t*)a.q + (long long)(s.q0 + tq) * a.q_stride + (size_t)(head * a.group + hh) * D + 4 * c;
-      float scale_row = 1.0f;
-      if (!BF16) {
 #pragma unroll
-        for (int i = 0; i < C::KSTEPS; ++i) {
-          const uint2 v = on ? *(const uint2*)(qrow + 16 * i) : make_uint2(0, 0);
-          qf[t][i][0] = v.x;
-          qf[t][i][1] = v.y;
-        }
-      } else {
-        uint2 v[C::KSTEPS];
+      for (int i = 0; i < C::KSTEPS; ++i) {
+        const uint2 v = on ? *(const uint2*)(qrow + 16 * i) : make_uint2(0, 0);
+        qf[t][i][0] = v.x;
+        qf[t][i][1] = v.y;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < C::STAGES - 1; ++j) {
+      const Place pg = pg_next;
+      pg_next = page_of(j + 1);
+      issue(j, pg);
+    }
+
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float scale_row = 1.0f;
+      if (BF16) {
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < C::KSTEPS; ++i) {
-          v[i] = on ? *(const uint2*)(qrow + 16 * i) : make_uint2(0, 0);
-          top = __vmaxu2(top, __vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu));
-        }
+        for (int i = 0; i < C::KSTEPS; ++i)
+          top = __vmaxu2(top, __vmaxu2(qf[t][i][0] & 0x7FFF7FFFu, qf[t][i][1] & 0x7FFF7FFFu));
         top = max(top & 0xFFFFu, top >> 16);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         float up;
         bf16_row_scale(top, up, scale_row);
 #pragma unroll
-        for (int i = 0; i < C::KSTEPS; ++i) {
-          const uint32_t w[2] = {v[i].x, v[i].y};
+        for (int i = 0; i < C::KSTEPS; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) qf[t][i][j] = bf16x2_to_h2(w[j], up);
-        }
+          for (int j = 0; j < 2; ++j) qf[t][i][j] = bf16x2_to_h2(qf[t][i][j], up);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -298,14 +322,14 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
       }
 
     for (int j = 0; j < mine_n; ++j) {
-      cp_async_wait<AB_STAGES - 2>();
+      cp_async_wait<C::STAGES - 2>();
       __syncwarp();
       {
-        const int pg = pg_next;
-        pg_next = page_of(j + AB_STAGES);
-        issue(j + AB_STAGES - 1, pg);
+        const Place pg = pg_next;
+        pg_next = page_of(j + C::STAGES);
+        issue(j + C::STAGES - 1, pg);
       }
-      const uint32_t st = ring + (j % AB_STAGES) * C::STAGE;
+      const uint32_t st = ring + (j % C::STAGES) * C::STAGE;
       const int p0 = position(j);
       const float sk = __uint_as_float(lds32(st + 2 * C::SIDE)), sv = __uint_as_float(lds32(st + 2 * C::SIDE + 4));
       // scores
@@ -332,17 +356,24 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
       const bool bad = sv < 0.0f;
       const float svc = fmaxf(sv, 1e-30f), lv = lg2(svc), inv_sv = __frcp_rn(svc);
       const bool partial = bad || p0 + 16 > all_see;
-      bool over = false;
+      float y[NT][4], most = -INFINITY;  // X - m
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        const float f0 = fs[t][0] * sk, f1 = fs[t][1] * sk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[t][i] = fmaf(x[t][i], i & 1 ? f1 : f0, lv);
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (bad || p0 + g + (i >> 1) * 8 >= lim[t][i & 1]) x[t][i] = -INFINITY;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[t][i] = fmaf(x[t][i], fs[t][i & 1] * sk, lv);
-          if (partial && (bad || p0 + g + (i >> 1) * 8 >= lim[t][i & 1])) x[t][i] = -INFINITY;
-          over = over || x[t][i] > m[t][i & 1] + AB_SLACK;
+          y[t][i] = x[t][i] - m[t][i & 1];
+          most = fmaxf(most, y[t][i]);
         }
       }
-      if (__any_sync(0xffffffffu, over)) {
+      if (__any_sync(0xffffffffu, most > AB_SLACK)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -360,6 +391,8 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
               acc[k][t][i] *= f;
               acc[k][t][i + 2] *= f;
             }
+            y[t][i] = x[t][i] - mn;
+            y[t][i + 2] = x[t][i + 2] - mn;
           }
       }
       uint32_t pf[NT][2];
@@ -368,7 +401,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          w[i] = ex2(x[t][i] - m[t][i & 1]);
+          w[i] = ex2(y[t][i]);
           l[t][i & 1] = fmaf(w[i], inv_sv, l[t][i & 1]);
         }
         // rounded to halves: 2^-12 of a weight at most on average over many positions, as exact as the FP16 output
