@@ -65,3 +65,23 @@ def test_write_of_no_tokens_is_no_launch():
     dict(workspace=A + 16, workspace_bytes=1 << 30), dict(max_q=1 << 30)], ids=str)
 def test_attention_refusals(change):
     refused(w4.attention_b8_paged, ATTEND, **change)
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 2), (1, 3, 2), (1, 0, 2), (1, 4, 0), (-5, 4, 2)], ids=str)
+def test_workspace_refusals(shape):
+    with pytest.raises(w4.InvalidArgument):
+        w4.attention_b8_workspace(*shape)
+
+
+def test_binding_refuses_what_the_abi_cannot_hold():
+    """The binding of these entries checks its integers instead of cutting them off."""
+    with pytest.raises(OverflowError):
+        w4.page_tables(**{**TABLES, "nseq": 1 << 31})
+    with pytest.raises(OverflowError):
+        w4.kv_write_b8(**{**WRITE, "T": 1 << 40})
+    with pytest.raises(OverflowError):
+        w4.attention_b8_paged(**{**ATTEND, "q": -1})
+    with pytest.raises(TypeError):
+        w4.attention_b8_paged(**{**ATTEND, "max_q": 1.5})
+    with pytest.raises(TypeError):
+        w4.page_tables(**{**TABLES, "bt": "table"})
