@@ -182,7 +182,7 @@ cudaError_t page_tables_launch(const PageTables& a, cudaStream_t stream) {
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;  // (a single CTA is a cluster of its own)
   return cudaLaunchKernelEx(&cfg, page_tables_kernel, a);
 }
 
