@@ -295,7 +295,8 @@ int w4b_attn_single_w4(const w4b_kv_w4* p, const void* q, void* out, void* strea
 
 /* No counterpart in the reference. The three calls of a serving step over a paged cache whose
  * lengths live on the device: the tables of the step, the write of the new tokens, attention.
- * All three only launch on `stream` and may be captured into a graph.
+ * All three only launch on `stream` and may be captured into a graph (the library's first call on a
+ * device allocates its status word: make one before the capture).
  *
  * w4b_page_tables: block tables and slot maps from request lengths. Request i (of nseq <= 16384)
  *   holds cached[i] positions and brings fresh[i] new tokens. Its new pages are taken from
