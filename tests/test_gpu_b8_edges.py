@@ -1,0 +1,68 @@
+"""GPU tests of the paged 8-bit cache operators at the edges of what a call may say: bounds above and below what the
+device-side counts ask for, table sizes around the shared memory's limits, values at the ends of their types. The plain
+forms and the tolerances are those of test_gpu_b8.py; what a test adds to them it derives where it stands."""
+import math
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+import w4a16_dequant_gemm_b200 as w4
+from test_gpu_b8 import BF16, CODE, F16, Problem, ints, plain_tables, run_tables, same_tables, stream, table_case
+
+pytestmark = pytest.mark.gpu
+
+
+def check_rows(p, out, lse, tokens, missing=()):
+    """`tokens` of the problem against its 64-bit form; all other rows as they were."""
+    ref, ref_lse, b_out, b_lse = p.reference(missing)
+    o, s = out[tokens].double().cpu(), lse[tokens].double().cpu()
+    empty = ref_lse[tokens] == -math.inf
+    assert (s[empty] == -math.inf).all() and (o[empty] == 0).all()
+    assert ((o - ref[tokens]).abs() <= b_out[tokens])[~empty].all()
+    assert ((s - ref_lse[tokens]).abs() <= b_lse[tokens])[~empty].all()
+    rest = torch.ones(len(out), dtype=torch.bool)
+    rest[tokens] = False
+    assert (out[rest.cuda()] == 9).all() and (lse[rest.cuda()] == 9).all()
+
+
+# ---- attention: max_q and max_seq_len are bounds -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("hkv,group,d", [(2, 4, 128), (2, 1, 64), (1, 40, 64)])
+@pytest.mark.parametrize("n", [0, 1, 5, 8, 9, 32, 33])
+def test_attention_max_q_above_every_count(n, hkv, group, d, dtype):
+    """max_q = 64 whatever the counts: one sequence alone, and beside an empty and a short one."""
+    for lens, nq in (([200 + n], [n]), ([100 + n, 0, 77], [n, 0, 2])):
+        p = Problem(lens, nq, hkv, group, d, 32, dtype, True, seed=300 + n)
+        p.check(*p.run(max_q=64))
+    assert w4.device_status() == 0
+
+
+@pytest.mark.parametrize("group", [1, 4])
+def test_attention_counts_change_between_replays(group):
+    """One captured call for up to 64 tokens of one request; the counts are written between its replays."""
+    p = Problem([300], [64], 2, group, 128, 16, F16, True, seed=320)
+    size = w4.attention_b8_workspace(64, 2 * group, 2)
+    ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    codes, hq = p.cache(), 2 * group
+    out, lse = torch.empty(66, hq, 128, dtype=F16, device="cuda"), torch.empty(66, hq, device="cuda")
+    dl, do = ints([300]), ints([0, 64])
+    desc = w4.DeviceKVB8(2, 128, 16, p.npages, codes[0].data_ptr(), p.scales[0].data_ptr(), codes[1].data_ptr(), p.scales[1].data_ptr())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w4.attention_b8_paged(desc, p.bt.data_ptr(), p.bt.stride(0), dl.data_ptr(), do.data_ptr(), 1, 64, 300, p.q.data_ptr(),
+                              p.q.stride(0), hq, w4.DTYPE_F16, out.data_ptr(), out.stride(0), lse.data_ptr(),
+                              workspace=ws.data_ptr(), workspace_bytes=size, stream=stream())
+    for n in (1, 64, 5, 0, 33, 9, 32, 64):
+        p.nq, p.offsets, p.tokens = [n], [0, n], n
+        do.copy_(ints([0, n]))
+        out.fill_(9)
+        lse.fill_(9)
+        graph.replay()
+        p.check(out, lse)
+    assert w4.device_status() == 0

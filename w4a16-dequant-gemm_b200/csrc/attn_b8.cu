@@ -629,8 +629,11 @@ cudaError_t attn_b8_launch(const AttnB8& args, int D, int bf16, int sm_count, cu
   *launches = 1;
   if (rows >= a.chunk_rows) {
     const cudaError_t e = attn_b8_chunk_launch(a, D, bf16, sm_count, stream);
-    // one sequence, or no row count below the threshold: nothing is left for the kernel below
-    if (e != cudaSuccess || a.nseq == 1) return e;
+    // The counts are on the device, max_q only bounds them: unless a single token already reaches the threshold, a
+    // sequence may be the kernel's below, also when there is only one. (That costs one long sequence 2 us. The chunk
+    // kernel taking a sequence alone whatever its count would cost a short one under a large max_q, 32 heads on 8 of
+    // 128: 1 token on 777 / 131,072 positions 23 / 178 us instead of 14 / 79.)
+    if (e != cudaSuccess || a.group >= a.chunk_rows) return e;
     *launches = 2;
     a.after_chunk = 1;
   }
