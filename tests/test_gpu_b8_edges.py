@@ -66,3 +66,15 @@ def test_attention_counts_change_between_replays(group):
         graph.replay()
         p.check(out, lse)
     assert w4.device_status() == 0
+
+
+# ---- block tables --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n", [4051, 4052, 4053, 4095, 4096, 9001, 16384])
+def test_tables_of_many_requests(n):
+    """Around 48 KB of shared memory (12 n + 8 bytes and what the kernel holds besides), and the most there may be."""
+    rng = np.random.default_rng(n)
+    cached, fresh, page, npages, free, bt, need = table_case(rng, n, 16, 40, 2)
+    tokens = sum(fresh)
+    same_tables((cached, fresh, page, npages, free, 0, bt, tokens + 5))
+    same_tables((cached, fresh, page, npages, free, 0, bt, tokens + 3), in_place=True)

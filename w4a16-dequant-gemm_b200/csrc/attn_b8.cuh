@@ -3,8 +3,6 @@
 
 #include <cuda_bf16.h>
 
-#include <atomic>
-
 #include "w4b_common.cuh"
 #include "w4b_kernels.h"
 
@@ -83,18 +81,6 @@ __device__ __forceinline__ int unit_owner(long long u, long long T, long long G)
 __device__ __forceinline__ long long range_begin(long long T, long long c, long long G) {
   const unsigned long long n = (unsigned long long)T * (unsigned long long)c;
   return n < 0x100000000ULL ? (long long)((unsigned)n / (unsigned)G) : (long long)(n / (unsigned long long)G);
-}
-
-// Opts a kernel into `bytes` of shared memory, once per device (the call costs as much as half a launch).
-template <auto kernel>
-cudaError_t opt_in_smem(int bytes) {
-  static std::atomic<bool> done[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || (dev < 64 && done[dev].load(std::memory_order_acquire))) return e;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_release);
-  return e;
 }
 
 }  // namespace w4b

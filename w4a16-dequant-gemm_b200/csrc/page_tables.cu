@@ -162,11 +162,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) page_tables_kernel(const PageTa
 
 cudaError_t page_tables_launch(const PageTables& a, cudaStream_t stream) {
   const size_t smem = ((size_t)3 * a.nseq + 2) * sizeof(int);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)((3 * kMaxTableRequests + 2) * sizeof(int)));
-    if (e != cudaSuccess) return e;
-  }
+  // always: what a launch may use without it is 48 KB together with the kernel's static shared memory
+  const cudaError_t e = opt_in_smem<page_tables_kernel>((int)((3 * kMaxTableRequests + 2) * sizeof(int)));
+  if (e != cudaSuccess) return e;
   // as many CTAs as the tokens or requests fill, up to one cluster
   const long long fill = ((long long)a.max_tokens / PT_TOKENS > a.nseq ? a.max_tokens / PT_TOKENS : a.nseq);
   int ctas = 1;

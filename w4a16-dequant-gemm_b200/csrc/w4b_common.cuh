@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "w4b_kernels.h"
 
 namespace w4b {
@@ -398,6 +400,18 @@ __device__ __forceinline__ uint4 pair_permute(uint4 v) {
   r.z = __byte_perm(v.y, v.w, 0x5410);
   r.w = __byte_perm(v.y, v.w, 0x7632);
   return r;
+}
+
+// Opts a kernel into `bytes` of shared memory, once per device (the call costs as much as half a launch).
+template <auto kernel>
+cudaError_t opt_in_smem(int bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && done[dev].load(std::memory_order_acquire))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_release);
+  return e;
 }
 
 }  // namespace w4b
