@@ -334,7 +334,9 @@ int w4b_attn_single_w4(const w4b_kv_w4* p, const void* q, void* out, void* strea
  *   lse (optional) [token][Hq] FP32, the natural log of the sum of exponentials. A token that sees
  *   nothing gets zeros and -inf. Rows of out outside the sequences' tokens are left as they are.
  *   A block-table entry outside 0..npages-1 is read as a page without positions (status 604).
- *   Lengths above max_seq_len and tokens above max_q are cut off there.
+ *   max_q and max_seq_len bound the counts on the device. Positions from max_seq_len on are not
+ *   attended to and a sequence's tokens from max_q on get no output (status 605); the other
+ *   tokens stand, and see, where seq_lens and q_offsets put them.
  *   ws: w4b_attn_b8_workspace(max_q, Hq, H) bytes of device memory for this call (256-byte aligned, zero-filled
  *   once by the caller; every call leaves the zeros it needs). Calls that may overlap - on two
  *   streams, or two captured graphs - take different ones. NULL: library scratch, which is

@@ -78,3 +78,32 @@ def test_tables_of_many_requests(n):
     tokens = sum(fresh)
     same_tables((cached, fresh, page, npages, free, 0, bt, tokens + 5))
     same_tables((cached, fresh, page, npages, free, 0, bt, tokens + 3), in_place=True)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "cross"])
+@pytest.mark.parametrize("nq,max_q,group", [([5, 2, 4], 3, 4), ([9], 1, 2), ([90, 20, 300], 40, 4), ([150], 70, 2), ([40, 3], 30, 1)], ids=str)
+def test_attention_more_tokens_than_max_q(nq, max_q, group, causal, dtype):
+    """The tokens behind the first max_q of a sequence are left out and reported; the others see what they would see."""
+    lens = [300 + 7 * n for n in nq]
+    p = Problem(lens, nq, 2, group, 128, 16, dtype, causal, seed=330)
+    out, lse = p.run(max_q=max_q)
+    kept = [p.offsets[i] + j for i, n in enumerate(nq) for j in range(min(n, max_q))]
+    check_rows(p, out, lse, kept)
+    assert w4.device_status() == 605
+    p.check(*p.run(max_q=max(nq)))
+    assert w4.device_status() == 0
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "cross"])
+@pytest.mark.parametrize("nq", [[1, 3], [60, 100], [130]], ids=str)
+def test_attention_longer_than_max_seq_len(nq, causal):
+    """Positions from max_seq_len on are left out and reported; a token's own position stays what it is."""
+    cut, page = 192, 16
+    lens = [250, 190][: len(nq)]
+    p = Problem(lens, nq, 2, 2, 64, page, F16, causal, seed=340)
+    p.max_len = cut
+    out, lse = p.run()
+    missing = [(i, c) for i in range(len(nq)) for c in range(cut // page, 20)]
+    check_rows(p, out, lse, list(range(p.tokens)), missing)
+    assert w4.device_status() == 605

@@ -194,8 +194,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
     const int rows = min(NC, s.nq * a.group - tile * NC);   // query rows in this tile
     const int tq0 = tile * NC / a.group;                      // first and last query token of the tile
     const int tq1 = (tile * NC + rows - 1) / a.group;
-    const int end = a.causal ? min(s.len, max(0, s.len - s.nq + tq1 + 1)) : s.len;  // positions any row sees
-    const int all_see = a.causal ? max(0, s.len - s.nq + tq0 + 1) : s.len;          // positions every row sees
+    const int end = positions_seen(a, s, tq1), all_see = positions_seen(a, s, tq0);  // seen by any row, by every row
     const int p_begin = r0 * AB_UNIT, p_end = min(r1 * AB_UNIT, end);
     const int nblocks = p_end > p_begin ? (p_end - p_begin + 15) / 16 : 0;
     const int mine_n = nblocks > wid ? (nblocks - wid + AB_WARPS - 1) / AB_WARPS : 0;
@@ -301,7 +300,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
         const int col = 2 * c + j;
         fs[t][j] = __shfl_sync(0xffffffffu, scale_row, col * 4) * (a.scale * AB_LOG2E);
         const int rr = tile * NC + t * 8 + col;
-        lim[t][j] = t * 8 + col < rows ? (a.causal ? s.len - s.nq + rr / a.group + 1 : s.len) : 0;
+        lim[t][j] = t * 8 + col < rows ? positions_seen(a, s, rr / a.group) : 0;
       }
     }
 

@@ -60,16 +60,26 @@ __device__ __forceinline__ uint32_t pack_out(float x, float y) {
 __device__ __forceinline__ float row_norm(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * AB_LN2; }
 
-// What a sequence asks for, with the device-side values held inside what the launch was sized for.
+// What a sequence asks for, with the device-side values held inside what the launch was sized for: positions from
+// max_len on and tokens from max_q on are left out (status), but where a token stands goes by the values as they are.
 struct SeqInfo {
   int len, q0, nq;
+  int first;  // causal: position of token 0 (negative when there are more tokens than positions)
 };
 __device__ __forceinline__ SeqInfo seq_info(const AttnB8& a, int i) {
   SeqInfo s;
-  s.len = min(max(a.seq_lens[i], 0), a.max_len);
+  const int len = max(a.seq_lens[i], 0);
   s.q0 = a.q_offsets ? a.q_offsets[i] : i;
-  s.nq = a.q_offsets ? min(max(a.q_offsets[i + 1] - s.q0, 0), a.max_q) : 1;
+  const int nq = a.q_offsets ? max(a.q_offsets[i + 1] - s.q0, 0) : 1;
+  s.len = min(len, a.max_len);
+  s.nq = min(nq, a.max_q);
+  s.first = len - nq;
+  if (len > a.max_len || nq > a.max_q) atomicExch(a.status, ST_ATTN_BOUNDS);
   return s;
+}
+// the positions token `tq` sees
+__device__ __forceinline__ int positions_seen(const AttnB8& a, const SeqInfo& s, int tq) {
+  return a.causal ? min(s.len, max(0, s.first + tq + 1)) : s.len;
 }
 
 // The split of T units over G CTAs: CTA c has units [T c / G, T (c + 1) / G), and unit u is CTA ((u + 1) G - 1) / T's.

@@ -151,7 +151,7 @@ __device__ __forceinline__ RowGroup row_group(const AttnB8& a, const SeqInfo& s,
   const int first = gi * AC_GROUP;
   t.rows = min(AC_GROUP, s.nq * a.group - first);
   t.split = t.rows <= AC_ROWS;
-  const int end = a.causal ? min(s.len, max(0, s.len - s.nq + (first + t.rows - 1) / a.group + 1)) : s.len;
+  const int end = positions_seen(a, s, (first + t.rows - 1) / a.group);
   t.tiles = max(1, (end + AC_TILE - 1) / AC_TILE);
   t.units = (t.split ? (t.tiles + 1) / 2 : t.tiles) + AC_ROW_COST;
   return t;
@@ -162,7 +162,7 @@ __device__ __forceinline__ int row_groups(const AttnB8& a, const SeqInfo& s) {
 }
 // Units of sequences i0 + lane (lane < n <= 32), all heads: a sequence of many groups by the whole warp, 32 at a time.
 __device__ __forceinline__ long long warp_units(const AttnB8& a, int i0, int n, int lane) {
-  SeqInfo s = {0, 0, 0};
+  SeqInfo s = {0, 0, 0, 0};
   if (lane < n) s = seq_info(a, i0 + lane);
   const int groups = row_groups(a, s);
   int mine = 0;
@@ -170,7 +170,8 @@ __device__ __forceinline__ long long warp_units(const AttnB8& a, int i0, int n, 
     for (int gi = 0; gi < groups; ++gi) mine += row_group(a, s, gi).units;
   for (uint32_t big = __ballot_sync(0xffffffffu, groups > 8); big != 0; big &= big - 1) {
     const int k = __ffs(big) - 1, all = __shfl_sync(0xffffffffu, groups, k);
-    const SeqInfo t = {__shfl_sync(0xffffffffu, s.len, k), 0, __shfl_sync(0xffffffffu, s.nq, k)};
+    const SeqInfo t = {__shfl_sync(0xffffffffu, s.len, k), 0, __shfl_sync(0xffffffffu, s.nq, k),
+                       __shfl_sync(0xffffffffu, s.first, k)};
     int sum = 0;
     for (int gi = lane; gi < all; gi += 32) sum += row_group(a, t, gi).units;
     sum = __reduce_add_sync(0xffffffffu, sum);
@@ -580,8 +581,8 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
       const int row_in = rt + (t.split ? 0 : AC_ROWS * w), row = k.gi * AC_GROUP + row_in;
       const bool on = row_in < t.rows;
       const int tq = on ? row / a.group : 0, hq = head * a.group + (on ? row - tq * a.group : 0);
-      const int lim = !on ? 0 : (a.causal ? s.len - s.nq + tq + 1 : s.len);
-      const int all_see = a.causal ? s.len - s.nq + (row - rt) / a.group + 1 : s.len;  // positions all its rows see
+      const int lim = on ? positions_seen(a, s, tq) : 0;
+      const int all_see = positions_seen(a, s, (row - rt) / a.group);  // positions all rows of the warpgroup see
       const int j_first = t.split ? w : 0, j_step = t.split ? 2 : 1;
       // this warp's accesses to tensor memory are done: tell the issuing thread
       auto signal = [&](uint32_t bar) {

@@ -32,6 +32,7 @@ enum : int {
   ST_PAGES_INVALID = 602,         // page tables: a negative count, a request longer than its table row, too many tokens
   ST_KV_WRITE_SLOT = 603,         // 8-bit cache write: a slot outside the pool, or a page's tokens out of order
   ST_KV_PAGE = 604,               // 8-bit attention: a block-table entry outside the pool (its positions are left out)
+  ST_ATTN_BOUNDS = 605,           // 8-bit attention: a length above max_seq_len or more tokens than max_q (left out)
 };
 
 // --------------------------------------------------------------------------
