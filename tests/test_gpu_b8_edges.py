@@ -107,3 +107,56 @@ def test_attention_longer_than_max_seq_len(nq, causal):
     missing = [(i, c) for i in range(len(nq)) for c in range(cut // page, 20)]
     check_rows(p, out, lse, list(range(p.tokens)), missing)
     assert w4.device_status() == 605
+
+
+# ---- the library's scratch -----------------------------------------------------------------------------------------
+
+SCRATCH = """
+import sys, threading, torch
+sys.path[:0] = ["tests", "."]
+import w4a16_dequant_gemm_b200 as w4
+from test_gpu_b8 import Problem, F16
+"""
+
+
+def in_a_fresh_process(script):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", SCRATCH + script], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+def test_scratch_is_complete_after_the_first_call():
+    """A process whose first call is a decode step, then captures a step of prompt chunks, both without a workspace."""
+    in_a_fresh_process("""
+one = Problem([500, 40], [1, 1], 2, 4, 128, 16, F16, True, seed=1)
+one.check(*one.run())
+p = Problem([500, 90], [70, 40], 2, 4, 128, 16, F16, True, seed=2)
+hq, codes = 8, p.cache()
+out, lse = torch.full((p.tokens + 2, hq, 128), 9.0, dtype=F16, device="cuda"), torch.full((p.tokens + 2, hq), 9.0, device="cuda")
+dl, do = torch.tensor(p.lens, dtype=torch.int32, device="cuda"), torch.tensor(p.offsets, dtype=torch.int32, device="cuda")
+desc = w4.DeviceKVB8(2, 128, 16, p.npages, codes[0].data_ptr(), p.scales[0].data_ptr(), codes[1].data_ptr(), p.scales[1].data_ptr())
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    w4.attention_b8_paged(desc, p.bt.data_ptr(), p.bt.stride(0), dl.data_ptr(), do.data_ptr(), 2, 70, 500, p.q.data_ptr(), p.q.stride(0),
+                          hq, w4.DTYPE_F16, out.data_ptr(), out.stride(0), lse.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+graph.replay()
+p.check(out, lse)
+""")
+
+
+def test_scratch_with_first_calls_of_several_threads():
+    """Eight threads make their first calls at once (on one stream, as calls without a workspace have to be)."""
+    in_a_fresh_process("""
+probs = [Problem([500 + 30 * i, 40], [n, 1], 2, 4, 128, 16, F16, True, seed=i) for i, n in enumerate([1, 60, 1, 200, 3, 90, 1, 64])]
+torch.cuda.synchronize()
+got, gate = [None] * len(probs), threading.Barrier(len(probs))
+def work(i):
+    gate.wait()
+    got[i] = probs[i].run()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(len(probs))]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for p, g in zip(probs, got):
+    p.check(*g)
+""")

@@ -83,7 +83,7 @@ struct DeviceCtx {
   Scratch attn_ws;        // (m, l, acc[D]) partials of split sequences
   Scratch io_x, io_c;     // device staging of the host-buffer entry
   Scratch gemm_xpad;      // zero-padded activation rows of the padded-K entries
-  Scratch b8_ws, b8_chunk_ws;  // counters and partial results of the 8-bit paged attention: one size, never replaced
+  Scratch b8_ws;          // counters and partial results of the 8-bit paged attention: one size, never replaced
 };
 
 constexpr int kMaxDevices = 64;
@@ -813,15 +813,13 @@ int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const in
   if (int rc = get_ctx(&ctx)) return rc;
   const bool chunked = b8_chunked(max_q, Hq / p->H);
   const size_t first = b8_ws_part(ctx->sm_count), second = chunked ? attn_b8_chunk_ws_bytes(ctx->sm_count) : 0;
-  void* chunk_ws = nullptr;
   if (ws) {
     if (ws_bytes < (long long)(first + second)) INVALID("%s: workspace of %lld bytes, %zu are needed", who, ws_bytes, first + second);
-    chunk_ws = (uint8_t*)ws + first;
   } else {
-    CUDA_TRY(ctx->b8_ws.reserve(first, true), "attention workspace");
-    CUDA_TRY(ctx->b8_chunk_ws.reserve(second, true), "attention workspace");
+    // whole at the first call, whatever its shape (later ones may be captured), and by one thread
+    std::lock_guard<std::mutex> lk(g_mu);
+    CUDA_TRY(ctx->b8_ws.reserve(first + attn_b8_chunk_ws_bytes(ctx->sm_count), true), "attention workspace");
     ws = ctx->b8_ws.ptr;
-    chunk_ws = ctx->b8_chunk_ws.ptr;
   }
   AttnB8 a;
   memset(&a, 0, sizeof(a));
@@ -848,7 +846,7 @@ int w4b_attn_b8_paged(const w4b_kv_b8* p, const int* bt, int bt_stride, const in
   a.out_stride = out_stride;
   a.lse = lse;
   a.ws = ws;
-  a.chunk_ws = chunk_ws;
+  a.chunk_ws = (uint8_t*)ws + first;
   a.chunk_rows = kChunkRows;
   a.page_div = FastDiv::of(p->page);
   a.status = ctx->status;
