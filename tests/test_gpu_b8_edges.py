@@ -160,3 +160,32 @@ threads = [threading.Thread(target=work, args=(i,)) for i in range(len(probs))]
 for p, g in zip(probs, got):
     p.check(*g)
 """)
+
+
+# ---- attention: values ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq,nseq", [(1, 80), (4, 80), (64, 20)])
+def test_attention_first_position_outweighs_all_others(nq, nseq, dtype):
+    """A first position e^18.75 = 2^27 above the others, whose own value is zero: the output is made of the others alone,
+    each weighing 2^-27 of it. With L positions, value v and e = exp(-18.75): out = v (L - 1) e / (1 + (L - 1) e). The
+    score is exact but for FP32 roundings (2^-19 of it, as elsewhere), the weights are rounded by 2^-11 relatively, or by
+    2^-34 of the largest one where that is more: half of the smallest half, 2^-25, beside a largest weight of 2^9 or more; lse = 18.75 + log(1 + (L - 1) e)."""
+    L, hkv, group, d, page, s, v = 2000, 8, 4, 64, 16, 18.75, 64.0
+    p = Problem([L] * nseq, [nq] * nseq, hkv, group, d, page, dtype, False, seed=350, scale=1.0)
+    codes = torch.zeros(2, hkv, p.npages, page, d, dtype=torch.uint8, device="cuda")
+    codes[1] = 0x68                                                   # 64
+    first = p.bt[:, 0].long()
+    codes[1][:, first, 0] = 0
+    codes[0][:, first, 0, 0] = 0x38                                   # 1
+    p.codes = codes.view(2, hkv, -1, d).view(torch.float8_e4m3fn)
+    p.scales.fill_(1.0)
+    p.q.zero_()
+    p.q[..., 0] = s
+    out, lse = p.run()
+    e = math.exp(-s)
+    want, want_lse = v * (L - 1) * e / (1 + (L - 1) * e), s + math.log1p((L - 1) * e)
+    half = 2.0 ** -11 if dtype == F16 else 2.0 ** -8
+    tol = want * (2.0 ** -11 + 2 * 2.0 ** -19 * s + 1.01 * half) + 2.0 ** -34 * L * v
+    assert ((out[:p.tokens].double() - want).abs() <= tol).all()
+    assert ((lse[:p.tokens].double() - want_lse).abs() <= 2.0 ** -19 * s + 2.0 ** -20 * (1 + want_lse)).all()

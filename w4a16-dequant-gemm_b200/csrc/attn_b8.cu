@@ -6,8 +6,8 @@
 //   w = 2^(X - m),  O^T[d][n] += sum_pos Vcode[pos][d] * w[pos][n],  l[n] += w / s_v
 // with m a reference point near the running maximum of X: taking log2(s_v) into the exponent puts V's scale into the
 // weights for free, whatever its size, and w / s_v is the plain softmax weight. out = O / l, lse = ln 2 (m + log2 l).
-// m moves only when some X exceeds it by more than 14 (a warp vote), so the usual block needs no reduction across
-// lanes: weights up to 2^14 are halves like others, and sums are FP32.
+// m moves only when some X exceeds it by more than 15 (a warp vote), so the usual block needs no reduction across
+// lanes: weights up to 2^15 are halves like others, and sums are FP32.
 //
 // Both products run on mma.sync.m16n8k16 with the CACHE as the 16-row operand and the query rows as the 8 columns
 // (a decode step has 1 to 16 rows: as the 128-row operand of the larger tensor instructions they would leave most of
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             // (only the columns that need it: a column's bits do not depend on the others')
-            const float mn = top > m[t][i] + AB_SLACK ? top : m[t][i], f = ex2(m[t][i] - mn);
+            const float mn = top > m[t][i] + AB_SLACK ? top - AB_BELOW : m[t][i], f = ex2(m[t][i] - mn);
             m[t][i] = mn;
             l[t][i] *= f;
 #pragma unroll
@@ -403,7 +403,9 @@ __global__ void __launch_bounds__(AB_THREADS, AB_CTAS_PER_SM) attn_b8_kernel(con
           w[i] = ex2(y[t][i]);
           l[t][i & 1] = fmaf(w[i], inv_sv, l[t][i & 1]);
         }
-        // rounded to halves: 2^-12 of a weight at most on average over many positions, as exact as the FP16 output
+        // rounded to halves, the type V's codes convert to exactly and both operands of the product share: off by at most
+        // 2^-11 of a weight, independently for each position, beside an output rounded by as much (FP16) or 2^-8 (BF16).
+        // The denominator sums them unrounded, so lse is as exact as the scores.
         pf[t][0] = movmatrix_trans(h2_as_u32(__floats2half2_rn(w[0], w[1])));
         pf[t][1] = movmatrix_trans(h2_as_u32(__floats2half2_rn(w[2], w[3])));
       }

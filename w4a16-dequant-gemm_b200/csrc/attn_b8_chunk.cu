@@ -9,7 +9,7 @@
 // A group of at most 128 rows is given to both warpgroups, which take the tiles in turn and join their results in
 // shared memory.
 //   warps 0-7   one thread per query row (its TMEM lane): no reduction across threads anywhere. The reference point m
-//               moves only when a score exceeds it by 2^14 (see attn_b8.cu); then O is rescaled in place.
+//               moves only when a score exceeds it by 2^15 (see attn_b8.cu); then O is rescaled in place.
 //   warps 8-11  E4M3 -> FP16 (exact), once for both warpgroups: 16-byte loads two tiles ahead in registers, written to
 //               swizzled operand tiles. K is K-major; V is stored the same way (row = position) and read MN-major.
 //   warp 12     one elected thread issues all MMAs: the scores of a warpgroup's next tile as soon as it has read the
@@ -689,7 +689,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
         for (int i = 0; i < AC_TILE; i += 2) top = max3(top, x.f[i], x.f[i + 1]);
         const bool move = bare ? top > -INFINITY : top > AB_SLACK;
         if (__any_sync(0xffffffffu, move)) {
-          const float by = move ? top : 0.0f, f = bare ? 0.0f : ex2(-by);  // (nothing to scale while bare)
+          const float by = move ? top - AB_BELOW : 0.0f, f = bare ? 0.0f : ex2(-by);  // (nothing to scale while bare)
           m += by;
           l *= f;
           bare = bare && !move;
