@@ -189,3 +189,45 @@ def test_attention_first_position_outweighs_all_others(nq, nseq, dtype):
     tol = want * (2.0 ** -11 + 2 * 2.0 ** -19 * s + 1.01 * half) + 2.0 ** -34 * L * v
     assert ((out[:p.tokens].double() - want).abs() <= tol).all()
     assert ((lse[:p.tokens].double() - want_lse).abs() <= 2.0 ** -19 * s + 2.0 ** -20 * (1 + want_lse)).all()
+
+
+def test_tables_in_place_keep_refused_requests():
+    """A loop that advances in place: a request that does not fit keeps its cached length and its pages, and goes on when
+    it is asked for something that fits."""
+    rng = np.random.default_rng(6)
+    cached, fresh, page, npages, free, bt, need = table_case(rng, 30, 16, 100, 30, spare=40)
+    cached[3] = max(cached[3], 20)
+    bt[3, :2] = free[-2:]
+    free = free[:-2]
+    fresh[3], fresh[7], cached[11] = page * bt.shape[1] + 1 - cached[3], -2, -4     # too long, negative counts
+    tokens = sum(max(f, 0) for f in fresh)
+    want = plain_tables(cached, fresh, page, npages, free, 0, bt, tokens)
+    got = run_tables(cached, fresh, page, npages, free, 0, bt, tokens, in_place=True)
+    refused = [3, 7, 11]
+    lens = [c if i in refused else n for i, (c, n) in enumerate(zip(cached, want[1]))]
+    assert got[6] == 602 and got[1] == lens
+    assert np.array_equal(want[0], got[0]) and list(want[2:6]) == list(got[2:6])
+    assert run_tables(cached, fresh, page, npages, free, 0, bt, tokens)[1] == want[1]   # into another array: 0
+    again = [1] * 30
+    again[11] = 0
+    same_tables((lens[:11] + [0] + lens[12:], again, page, npages, free, got[5], got[0], 40))
+
+
+def test_tables_in_place_go_on_after_the_pages_ran_out():
+    """A request that got no page for some positions: its length set back to its first missing entry, it goes on with
+    the pages of another list."""
+    rng = np.random.default_rng(7)
+    cached, fresh, page, npages, free, bt, need = table_case(rng, 20, 16, 100, 60, spare=80)
+    tokens = sum(fresh)
+    bt, lens, _, _, _, taken, status = run_tables(cached, fresh, page, npages, free[:need - 9], 0, bt, tokens, in_place=True)
+    assert status == 601 and taken == need - 9
+    for i, n in enumerate(lens):
+        gone = [c for c in range(-(-n // page)) if bt[i, c] < 0]
+        if gone:
+            assert gone[0] * page >= cached[i]
+            lens[i] = gone[0] * page
+    left = [cached[i] + fresh[i] - n for i, n in enumerate(lens)]
+    assert sum(left) > 0
+    want = plain_tables(cached, fresh, page, npages, free, 0, bt, tokens)   # as if they had been there at once
+    got = run_tables(lens, left, page, npages, free[need - 9:], 0, bt, sum(left), in_place=True)
+    assert got[6] == 0 and got[1] == want[1] and np.array_equal(got[0], want[0])
