@@ -327,7 +327,9 @@ int w4b_attn_single_w4(const w4b_kv_w4* p, const void* q, void* out, void* strea
  *   the scale when its values fit and else raises it the same way and rounds the page's earlier
  *   codes again. Rows behind the run keep their bytes. Status 501: a value that is not finite (that
  *   token's row of that head is written as zeros) or too large; 603: a slot outside the pool, or a
- *   page's tokens out of order (they are not written).
+ *   second run in a page, directly behind the first (a gap, a step back) or with skipped tokens
+ *   between them; it is not written. A page that comes back behind written tokens of other pages,
+ *   or behind page and more skipped ones, is not noticed: its codes are then undefined.
  * w4b_attn_b8_paged: softmax(scale * q k^T) v over the cache for the new tokens of nseq sequences.
  *   Hq query heads share the H cache heads in groups of Hq / H. Sequence i has seq_lens[i] <=
  *   max_seq_len positions (its new tokens included) and query tokens q_offsets[i] ..

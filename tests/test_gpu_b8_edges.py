@@ -231,3 +231,45 @@ def test_tables_in_place_go_on_after_the_pages_ran_out():
     want = plain_tables(cached, fresh, page, npages, free, 0, bt, tokens)   # as if they had been there at once
     got = run_tables(lens, left, page, npages, free[need - 9:], 0, bt, sum(left), in_place=True)
     assert got[6] == 0 and got[1] == want[1] and np.array_equal(got[0], want[0])
+
+
+# ---- the write -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("page", [16, 32, 48, 256])
+def test_write_refuses_a_page_that_comes_back(page):
+    """Slots of a page that stand apart - by tokens that are not written - are two runs of it: the first is written,
+    the second is reported and not written."""
+    H, D, npages = 2, 64, 8
+    b = [i * page for i in range(npages)]
+    cases = [
+        ([5, -1, 7], [0]),
+        ([5, -1, 6], [0]),
+        ([5, 10 ** 9, 6, 7], [0]),
+        ([b[1] + 4, 10 ** 9, -1, b[1] + 5, b[1] + 6], [0]),
+        ([b[2] + 3, b[2] + 4, -1, b[2], b[2] + 1, b[5]], [0, 1, 5]),
+        ([7] + [-1] * (page - 2) + [8], [0]),
+        ([b[4] + 2, -1, b[5] + 2, -1, b[4] + 1, b[6] + 2], [0, 2, 5]),
+    ]
+    for slots, kept in cases:
+        T = len(slots)
+        gen = torch.Generator().manual_seed(len(slots))
+        x = (torch.randn(2, T, H, D, generator=gen) + 3).to(F16).cuda()
+        got = []
+        for use in (slots, [s if i in kept else -1 for i, s in enumerate(slots)]):
+            q = torch.zeros(2, H, npages * page, D, dtype=torch.uint8, device="cuda")
+            sc = torch.full((2, H, npages), 2.0 ** -7, device="cuda")
+            sl = ints(use)
+            p = w4.DeviceKVB8(H, D, page, npages, q[0].data_ptr(), sc[0].data_ptr(), q[1].data_ptr(), sc[1].data_ptr())
+            w4.kv_write_b8(p, sl.data_ptr(), T, x[0].data_ptr(), x[1].data_ptr(), H * D, H * D, w4.DTYPE_F16, stream())
+            got.append((w4.device_status(), q.cpu(), sc.cpu()))
+        assert got[0][0] == 603 and got[1][0] == 0, slots
+        assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][2], got[1][2]), slots
+        assert (got[0][1] != 0).any(-1).any(1).any(0).nonzero().flatten().tolist() == sorted(slots[i] for i in kept)
+
+
+def test_write_takes_other_pages_in_any_order():
+    """Runs of different pages in any order, with skipped tokens between them, are all written."""
+    from test_gpu_b8 import new_rows, run_write, runs
+    slots = runs([(100, 12), (16, 16), (3, 13)]) + [-1, -1] + runs([(64, 5)]) + [-1] + runs([(53, 2), (80, 16), (40, 1)])
+    x = new_rows(len(slots), 2, 64, F16, 17)
+    run_write(2, 64, 16, 8, slots, x[0], x[1])

@@ -16,7 +16,7 @@
 // integers. A CTA looks for the runs that begin in its window of tokens and takes some of the 2 H (side, head) items of
 // each: finding a run is two dependent reads of the slot map, which a long step's CTAs share between several items.
 // Measured: 64 single tokens, 8 heads of 128, FP16: 3.3 us; 17,417 tokens, 8 heads of 128 out of rows of 12 KB, BF16:
-// 29.2 us = 3.7 TB/s, 0.56 of the measured copy rate (39.6 us with a CTA for every run and item). What is left there
+// 26.0 us = 4.1 TB/s, 0.63 of the measured copy rate (39.6 us with a CTA for every run and item). What is left there
 // are the instructions around each run and item; loads one item ahead cost more registers than they hid.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -73,6 +73,15 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
   return out;
 }
 
+// Whether one of the `reach` tokens before token t has a slot in the page that begins at row `base`. (Out of line: only
+// tokens behind skipped ones ask, and its instructions in the kernel's way cost a decode step 0.4 us of 3.3.)
+__device__ __noinline__ bool page_before(const int* slots, int t, int reach, unsigned base, unsigned page) {
+  bool found = false;
+#pragma unroll 4
+  for (int j = 1; j <= reach; ++j) found = found || (unsigned)slots[t - j] - base < page;
+  return found;
+}
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(512, KW_BLOCKS) kv_write_b8_kernel(const KvWriteB8 a) {
   constexpr int LPR = D / 8;  // lanes per row
@@ -108,6 +117,8 @@ __global__ void __launch_bounds__(512, KW_BLOCKS) kv_write_b8_kernel(const KvWri
         } else if (slot >= 0 && (slot % a.page == 0 || before != slot - 1)) {
           // a second run in the page of the token before: its scale would be a race
           wrong = before >= 0 && before / a.page == slot / a.page;
+          if ((before < 0 || before >= rows) && t > 1)  // behind tokens that are not written: as many as a page has rows
+            wrong = page_before(a.slots, t, min(a.page - 1, t), (unsigned)(slot - slot % a.page), (unsigned)a.page);
           head = !wrong;
         }
       }
