@@ -273,3 +273,14 @@ def test_write_takes_other_pages_in_any_order():
     slots = runs([(100, 12), (16, 16), (3, 13)]) + [-1, -1] + runs([(64, 5)]) + [-1] + runs([(53, 2), (80, 16), (40, 1)])
     x = new_rows(len(slots), 2, 64, F16, 17)
     run_write(2, 64, 16, 8, slots, x[0], x[1])
+
+
+@pytest.mark.parametrize("nq", [1, 5, 40])
+def test_attention_bf16_queries_at_the_ends_of_the_type(nq):
+    """Query values up to 2e38 and down to the subnormal ones, with scales that bring the scores back to a few units."""
+    p = Problem([300, 70], [nq, nq], 2, 2, 64, 16, BF16, True, seed=360, q_amp=4e37, scale=2e-38)
+    p.check(*p.run())
+    p = Problem([300, 70], [nq, nq], 2, 2, 128, 16, BF16, True, seed=361, q_amp=1e36, scale=1e-36)
+    p.check(*p.run())
+    p = Problem([300, 70], [nq, nq], 2, 2, 64, 16, BF16, True, seed=362, q_amp=1e-37, scale=1e29, scale_exp=(18, 21))
+    p.check(*p.run())

@@ -45,9 +45,11 @@ __device__ __forceinline__ float lg2(float x) {
 }
 
 // BF16 query rows become FP16 by a power of two of the row's own: with `top` the largest |q| (bits) its largest value
-// lands in [2^14, 2^15), and what falls below the half range is 2^-39 of it. scale_row undoes it in the scores.
+// lands in [2^14, 2^15), and what falls below the half range is 2^-39 of it. scale_row undoes it in the scores. The power
+// ends where one of the two would not be a normal number: at 2^-113 every finite row still fits, at 2^126 rows below
+// 2^-112 stay smaller, the smallest subnormal at 2^-7.
 __device__ __forceinline__ void bf16_row_scale(uint32_t top, float& up, float& scale_row) {
-  const int k = min(max(141 - (int)(top >> 7), -100), 100);  // 127 + 14 - the biased exponent
+  const int k = min(max(141 - (int)(top >> 7), -113), 126);  // 127 + 14 - the biased exponent
   up = __uint_as_float((uint32_t)(127 + k) << 23);
   scale_row = __uint_as_float((uint32_t)(127 - k) << 23);
 }

@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
           const bool on = w.sv >= 0.0f;
           const float v = fmaxf(w.sv, 1e-30f);
           *(float4*)(smp + L::META_OFF + ((it + j) % L::METAS * 4 + ct) * 16) =
-              make_float4(on ? w.sk * (a.scale * AB_LOG2E) : 0.0f, on ? lg2(v) : -INFINITY, on ? 1.0f / v : 0.0f, 0.0f);
+              make_float4(on ? w.sk : 0.0f, on ? lg2(v) : -INFINITY, on ? 1.0f / v : 0.0f, 0.0f);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -638,6 +638,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1) attn_b8_chunk_kernel(const Attn
           h[4 * p + 2] = BF16 ? bf16x2_to_h2(x.z, up) : x.z;
           h[4 * p + 3] = BF16 ? bf16x2_to_h2(x.w, up) : x.w;
         }
+        scale_row *= a.scale * AB_LOG2E;  // (in this order: a large row may come with a small scale, and the other way round)
         tmem_st32(t_q + lane_off, h);
         if (D == 128) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tmem_wait_st();
