@@ -284,3 +284,11 @@ def test_attention_bf16_queries_at_the_ends_of_the_type(nq):
     p.check(*p.run())
     p = Problem([300, 70], [nq, nq], 2, 2, 64, 16, BF16, True, seed=362, q_amp=1e-37, scale=1e29, scale_exp=(18, 21))
     p.check(*p.run())
+
+
+def test_tables_of_pages_near_2_to_31():
+    """One page of 2^31 - 1 positions: the tokens of a request that holds it go into it."""
+    page = 2 ** 31 - 1
+    for cached, fresh in ((5, 3), (2 ** 30 + 1, 2), (page - 1, 1), (0, 4)):
+        bt = np.full((1, 1), 0 if cached else -3, dtype=np.int32)
+        same_tables(([cached], [fresh], page, 1, [] if cached else [0], 0, bt, fresh + 1))

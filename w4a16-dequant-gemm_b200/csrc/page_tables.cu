@@ -33,6 +33,7 @@ __device__ __forceinline__ long long warp_inclusive(long long v, int lane) {
   return v;
 }
 
+__device__ __forceinline__ int pages_of(int n, int page) { return n / page + (n % page != 0); }  // (n + page may pass 2^31)
 __device__ __forceinline__ int clamp_int(long long v) { return v > INT_MAX ? INT_MAX : (int)v; }
 
 // The last i with off[i] <= v (off ascending, off[0] == 0 <= v).
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) page_tables_kernel(const PageTa
       f = max(0, fr);
       const bool fits = c >= 0 && fr >= 0 && (long long)c + fr <= room;
       bad = bad || !fits;
-      if (fits) need = (c + fr + (long long)a.page - 1) / a.page - (c + (long long)a.page - 1) / a.page;
+      if (fits) need = pages_of(c + fr, a.page) - pages_of(c, a.page);
       have[i] = fits ? c : -1;
     }
     const long long fi = warp_inclusive(f, lane), ni = warp_inclusive(need, lane);
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) page_tables_kernel(const PageTa
   };
   for (int j = gt; j < pg[a.nseq]; j += gn) {
     const int i = find_last(pg, a.nseq, j);
-    const int col = (have[i] + a.page - 1) / a.page + (j - pg[i]);
+    const int col = pages_of(have[i], a.page) + (j - pg[i]);
     a.bt[(long long)i * a.bt_stride + col] = listed((long long)taken + j);
   }
   const bool vec = ((((uintptr_t)a.slots | (uintptr_t)a.positions) & 15u) == 0);
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) page_tables_kernel(const PageTa
         while (tok[i + 1] <= t) ++i;  // ends: tok[nseq] > t
         if (have[i] >= 0) {
           pos[k] = have[i] + ((int)t - tok[i]);
-          const int col = pos[k] / a.page, first = (have[i] + a.page - 1) / a.page;
+          const int col = pos[k] / a.page, first = pages_of(have[i], a.page);
           int p;
           if (col >= first) {
             p = listed((long long)taken + pg[i] + (col - first));
