@@ -292,3 +292,14 @@ def test_tables_of_pages_near_2_to_31():
     for cached, fresh in ((5, 3), (2 ** 30 + 1, 2), (page - 1, 1), (0, 4)):
         bt = np.full((1, 1), 0 if cached else -3, dtype=np.int32)
         same_tables(([cached], [fresh], page, 1, [] if cached else [0], 0, bt, fresh + 1))
+
+
+def test_tables_with_token_sums_beyond_32_bits():
+    """Refused requests whose counts sum up past 2^31: the lengths of the requests behind them are their own."""
+    huge, page = 2 ** 31 - 1, 16
+    cached, fresh = [20, 5, 0, 33, 7], [3, huge, huge, 5, 30]
+    bt = np.array([[1, 2, -3, -3], [3, -3, -3, -3], [-3] * 4, [4, 5, 6, -3], [7, -3, -3, -3]], dtype=np.int32)
+    got = run_tables(cached, fresh, page, 64, list(range(20, 40)), 0, bt, 10)
+    assert got[6] == 602 and got[1] == [23, 0, 0, 38, 37]
+    assert got[0][4].tolist() == [7, 20, 21, -3] and got[5] == 2
+    assert got[3][:3] == [36, 37, 38] and got[3][3:] == [-1] * 7

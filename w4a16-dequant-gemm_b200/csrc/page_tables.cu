@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) page_tables_kernel(const PageTa
   for (int i = gt; i <= a.nseq; i += gn) {
     a.q_offsets[i] = tok[i];
     if (i == a.nseq) break;
-    if (have[i] >= 0) a.seq_lens[i] = have[i] + (tok[i + 1] - tok[i]);
+    if (have[i] >= 0) a.seq_lens[i] = have[i] + a.fresh[i];  // (not from the sums, which may have ended at 2^31 - 1)
     else if (a.seq_lens != a.cached) a.seq_lens[i] = 0;  // (in place the request keeps what it had)
   }
   // entry `at` of the free list, -1 behind its end or for a page the pool does not have
