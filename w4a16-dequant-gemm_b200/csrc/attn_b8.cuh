@@ -94,7 +94,7 @@ __device__ __forceinline__ int positions_seen(const AttnB8& a, const SeqInfo& s,
 // (64-bit division is some hundred instructions, so 32-bit where it suffices, and only where a row is split.)
 __device__ __forceinline__ int unit_owner(long long u, long long T, long long G) {
   const unsigned long long n = (unsigned long long)(u + 1) * (unsigned long long)G - 1;
-  return n < 0x100000000ULL ? (int)((unsigned)n / (unsigned)T) : (int)(n / (unsigned long long)T);
+  return (n | (unsigned long long)T) < 0x100000000ULL ? (int)((unsigned)n / (unsigned)T) : (int)(n / (unsigned long long)T);
 }
 __device__ __forceinline__ long long range_begin(long long T, long long c, long long G) {
   const unsigned long long n = (unsigned long long)T * (unsigned long long)c;

@@ -160,25 +160,6 @@ __device__ __forceinline__ int row_groups(const AttnB8& a, const SeqInfo& s) {
   const int rows = s.nq * a.group;
   return rows >= a.chunk_rows ? (rows + AC_GROUP - 1) / AC_GROUP : 0;
 }
-// Units of sequences i0 + lane (lane < n <= 32), all heads: a sequence of many groups by the whole warp, 32 at a time.
-__device__ __forceinline__ long long warp_units(const AttnB8& a, int i0, int n, int lane) {
-  SeqInfo s = {0, 0, 0, 0};
-  if (lane < n) s = seq_info(a, i0 + lane);
-  const int groups = row_groups(a, s);
-  int mine = 0;
-  if (groups <= 8)
-    for (int gi = 0; gi < groups; ++gi) mine += row_group(a, s, gi).units;
-  for (uint32_t big = __ballot_sync(0xffffffffu, groups > 8); big != 0; big &= big - 1) {
-    const int k = __ffs(big) - 1, all = __shfl_sync(0xffffffffu, groups, k);
-    const SeqInfo t = {__shfl_sync(0xffffffffu, s.len, k), 0, __shfl_sync(0xffffffffu, s.nq, k),
-                       __shfl_sync(0xffffffffu, s.first, k)};
-    int sum = 0;
-    for (int gi = lane; gi < all; gi += 32) sum += row_group(a, t, gi).units;
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == k) mine = sum;
-  }
-  return (long long)a.H * mine;
-}
 __device__ __forceinline__ long long warp_scan(long long v, int lane) {  // inclusive
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -186,6 +167,25 @@ __device__ __forceinline__ long long warp_scan(long long v, int lane) {  // incl
     if (lane >= d) v += o;
   }
   return v;
+}
+// Units of sequences i0 + lane (lane < n <= 32), all heads: a sequence of many groups by the whole warp, 32 at a time.
+__device__ __forceinline__ long long warp_units(const AttnB8& a, int i0, int n, int lane) {
+  SeqInfo s = {0, 0, 0, 0};
+  if (lane < n) s = seq_info(a, i0 + lane);
+  const int groups = row_groups(a, s);
+  long long mine = 0;  // (a prompt of a million tokens over millions of positions has more units than 32 bits hold)
+  if (groups <= 8)
+    for (int gi = 0; gi < groups; ++gi) mine += row_group(a, s, gi).units;
+  for (uint32_t big = __ballot_sync(0xffffffffu, groups > 8); big != 0; big &= big - 1) {
+    const int k = __ffs(big) - 1, all = __shfl_sync(0xffffffffu, groups, k);
+    const SeqInfo t = {__shfl_sync(0xffffffffu, s.len, k), 0, __shfl_sync(0xffffffffu, s.nq, k),
+                       __shfl_sync(0xffffffffu, s.first, k)};
+    long long sum = 0;
+    for (int gi = lane; gi < all; gi += 32) sum += row_group(a, t, gi).units;
+    sum = __shfl_sync(0xffffffffu, warp_scan(sum, lane), 31);
+    if (lane == k) mine = sum;
+  }
+  return a.H * mine;
 }
 
 template <int D>
