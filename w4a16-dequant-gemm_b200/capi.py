@@ -221,9 +221,6 @@ class DeviceKVB8:
     q_v: int
     s_v: int
 
-    def _c(self):
-        return _KvB8(self.H, self.D, self.page, self.npages, self.q_k, self.s_k, self.q_v, self.s_v)
-
 
 # ---- entry points, named as in the reference ------------------------------
 
