@@ -342,6 +342,8 @@ int w4b_attn_single_w4(const w4b_kv_w4* p, const void* q, void* out, void* strea
  *   halves before they meet the values, each off by at most 2^-11 of itself or, where that is more,
  *   2^-34 of the row's largest: 2^-11 of sum p |v| in out at most, and typically as much as an FP16
  *   output's own rounding. Rows of out outside the sequences' tokens are left as they are.
+ *   Masked positions weigh nothing, but a NaN code (0x7F, 0xFF; the write makes none) of V behind a
+ *   token still meets its row as 0 x NaN: every position below seq_lens is to have been written.
  *   A block-table entry outside 0..npages-1 is read as a page without positions (status 604).
  *   max_q and max_seq_len bound the counts on the device. Positions from max_seq_len on are not
  *   attended to and a sequence's tokens from max_q on get no output (status 605); the other

@@ -18,17 +18,19 @@
 //      conversions make the transposed operand (row g = dim 2g, row g + 8 = dim 2g + 1).
 // E4M3 -> FP16 is exact. The weights go from accumulator to operand layout by movmatrix.
 //
-// Bound by HBM: the cache is read once. Each warp keeps its own ring of 16-position blocks (K and V, 4 KB at D = 128)
-// filled by cp.async three blocks ahead, without any barrier between warps.
+// Bound by HBM: the cache is read once per column tile, so once for up to 16 query rows a head and twice for 17 to 32.
+// Each warp keeps its own ring of 16-position blocks (K and V, 4 KB at D = 128) filled by cp.async two blocks ahead
+// (D = 64: five), without any barrier between warps.
 //
 // Split: all work - 64-position units of all (sequence, head, column tile) rows in order - is cut into equal ranges,
 // one per CTA, whatever the lengths; the lengths are on the device, so every CTA sums them itself. A row that spans
 // CTAs is joined by whichever of them arrives last, in CTA order (bit-identical from run to run).
 //
 // Measured (device time in a graph): 4 sequences x 131,072 positions, 32 query heads on 8 of 128: 191 us = 5.6 TB/s,
-// 0.86 of the measured copy rate; 64 sequences of 100 to 8192 positions, 64 heads on 8 of 128: 55 us = 4.6 TB/s (0.69;
+// 0.86 of the measured copy rate; 64 sequences of 100 to 8192 positions, 64 heads on 8 of 128: 56 us = 4.5 TB/s (0.68;
 // 5 us of it are launch, the sums over the lengths and the first loads, 70 us without AB_ROW_COST: CTAs with many
-// short rows came late); one sequence of 778: 8 us.
+// short rows came late); one sequence of 778: 8.5 us. (The 16-column form at D = 128 spills 76 bytes: four CTAs an SM
+// leave 128 registers.)
 #include "attn_b8.cuh"
 
 namespace w4b {

@@ -24,12 +24,12 @@
 // Split: units of one tile (two, for a group that both warpgroups share) over all (sequence, head, row group) in
 // order, cut into equal ranges, as in attn_b8.cu; the causal limit of every group is in the count.
 //
-// Measured: 2 x 1k tokens on 4 to 6k positions, 32 query heads on 8 of 128, BF16: 207-211 us = 0.88-0.9 PFLOP/s, 0.54
+// Measured: 2 x 1k tokens on 4 to 6k positions, 32 query heads on 8 of 128, BF16: 210-214 us = 0.87-0.88 PFLOP/s, 0.53
 // of the measured matrix rate. A tile takes about 2200 cycles where its products take 1500 and its exponentials 1024:
 // what bounds it is the chain of one warpgroup - scores from tensor memory, maximum, exponentials, weights back - of
 // which only two run side by side. Tried without gain: a quarter to a half of the exponentials as polynomials on the
 // FMA pipe (215-228 against 218), holding the warpgroups half a tile apart (228), codes brought into L2 four tiles
-// ahead (212 against 207). A group costs about 8 us besides its tiles when it is split between CTAs.
+// ahead (212 against 207; all with the reference point at the maximum, attn_b8.cuh). A group costs about 8 us besides its tiles when it is split between CTAs.
 #include <cuda_bf16.h>
 #include <float.h>
 

@@ -17,7 +17,8 @@
 // each: finding a run is two dependent reads of the slot map, which a long step's CTAs share between several items.
 // Measured: 64 single tokens, 8 heads of 128, FP16: 3.3 us; 17,417 tokens, 8 heads of 128 out of rows of 12 KB, BF16:
 // 26.0 us = 4.1 TB/s, 0.63 of the measured copy rate (39.6 us with a CTA for every run and item). What is left there
-// are the instructions around each run and item; loads one item ahead cost more registers than they hid.
+// are the waits for each item's loads and the instructions around each run (issue 0.59, DRAM 0.37 of their peaks); loads
+// one item ahead in registers cost more of them than they hid, copies into shared memory were not tried.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -27,7 +28,7 @@
 namespace w4b {
 namespace {
 
-constexpr int KW_HELD = 8;            // 8-value pieces a thread keeps in registers (4: 30.4 us where 8 take 29.2)
+constexpr int KW_HELD = 8;            // 8-value pieces a thread keeps in registers (4: 34.8 us where 8 take 26.0)
 constexpr int KW_BLOCKS = 2;          // CTAs of 512 threads per SM: 64 registers a thread
 constexpr int KW_MIN_EXP = -60, KW_MAX_EXP = 60;
 
