@@ -73,7 +73,7 @@ struct Scratch {
 };
 
 struct DeviceCtx {
-  bool ready = false;
+  std::atomic<bool> ready{false};
   int sm_count = 0;
   int* status = nullptr;  // device status word written by bounded waits
   Scratch gemm_ws;        // FP32 partial fragments of split panels
@@ -106,6 +106,7 @@ int get_ctx(DeviceCtx** out) {
                     major);
       CUDA_TRY(cudaMalloc((void**)&c.status, sizeof(int)), "status word");
       CUDA_TRY(cudaMemset(c.status, 0, sizeof(int)), "status word");
+      CUDA_TRY(cudaStreamSynchronize(0), "status word");  // (the caller's stream need not be ordered behind it)
       c.ready = true;
     }
   }
