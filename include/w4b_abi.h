@@ -312,11 +312,13 @@ int w4b_attn_single_w4(const w4b_kv_w4* p, const void* q, void* out, void* strea
  *   word: 601 when the free list ends early (the missing entries and their tokens' slots are -1,
  *   *taken_out = nfree); 602 for a negative count, for a request longer than its table row or the
  *   pool (it gets no pages, its tokens slot -1, its seq_lens 0 - or, where seq_lens is cached, what
- *   it was), or when the tokens exceed max_tokens (the first max_tokens are mapped). For a loop that
- *   advances in place: a refused request is as before the step, only its outputs of the step mean
- *   nothing; a request that ran out of pages is sound up to its first -1 entry, so set its length
- *   back to that entry's first position before the next step (entries below the length are taken
- *   as held and not given again).
+ *   it was), or when the tokens exceed max_tokens (the first max_tokens are mapped; q_offsets go on
+ *   to the whole sum, and an attention call over them touches that many rows of q and out, so a
+ *   step whose sum is not known to fit is checked before it). For a loop that advances in place: a
+ *   refused request is as before the step, only its outputs of the step mean nothing; a request
+ *   that ran out of pages is sound up to its first -1 entry, so set its length back to that entry's
+ *   first position before the next step (entries below the length are taken as held and not given
+ *   again).
  * w4b_kv_write_b8: rows of T new tokens into the cache. k_new / v_new: FP16 or BF16 (dtype), token
  *   t's H*D values at t * k_stride / t * v_stride values (multiples of 8, so a fused projection can
  *   be passed as it is; bases 16-byte aligned). slots[t] is the token's row, -1 skips it. The tokens
